@@ -370,6 +370,36 @@ typedef struct LrceMhaDesc {
 int lrce_mha_fwd(const LrceMhaDesc* desc, void* stream);
 int lrce_mha_bwd(const LrceMhaDesc* desc, void* stream);
 
+/* Attention at general lengths: q [B][Lq][H][D], k / v [B][Lk][Hk][D] (16 bits: bf16, or IEEE fp16 with f16), H a
+ * multiple of Hk (query head h reads key head h / (H / Hk)), D 32, 64, 96 or 128, strides (batch, row, head) in
+ * elements, multiples of 8, the last axis contiguous, tensors 16-byte aligned.  out_i = sum_j softmax_j(scale q_i . k_j) v_j
+ * and lse [B][H][Lq] (f32, natural logarithm) over the keys that row i may see: key_mask [B][Lk] (entries of mask_bytes =
+ * 1, 4 or 8 bytes, 0 = hidden; NULL: all) and, with causal, j <= i + Lk - Lq.  A row that sees no key: out = 0, lse = -inf.
+ * What k and v hold at keys that key_mask hides, or behind Lk, enters no result (NaN included).  workspace:
+ * lrce_attn_fwd_workspace() / lrce_attn_bwd_workspace() floats (0: may be NULL, negative: bad descriptor).
+ * Backward: dq, dk, dv (stored) from dout and the forward's out and lse; the weights are recomputed. */
+typedef struct LrceAttnDesc {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const void* key_mask;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+  int64_t mask_stride;
+  int32_t B, H, Hk, Lq, Lk, D;
+  int32_t f16, causal, mask_bytes;
+  float scale;
+  float* workspace;
+  int64_t workspace_elems;
+  const void* dout;
+  void *dq, *dk, *dv;
+  int64_t g_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} LrceAttnDesc;
+
+int64_t lrce_attn_fwd_workspace(const LrceAttnDesc* desc);
+int64_t lrce_attn_bwd_workspace(const LrceAttnDesc* desc);
+int lrce_attn_fwd(const LrceAttnDesc* desc, void* stream);
+int lrce_attn_bwd(const LrceAttnDesc* desc, void* stream);
+
 /* ---------------------------------------------------------------- recurrent decoder attention blocks
  * One nn.TransformerDecoderLayer (fusionv3.py:8-17: d_model 768, 12 heads x 64, post-norm, one query
  * token per row) has two attention blocks that factor by head; each is ONE launch of B x 12

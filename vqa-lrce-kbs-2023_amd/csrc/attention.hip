@@ -1,0 +1,467 @@
+// Multi-head attention at general lengths on gfx950: head dims 32 / 64 / 96 / 128, bf16 or fp16, shared key / value
+// heads, a key mask and / or causality, forward.
+//
+//   s_ij = scale q_i . k_j,  m_i = max_j s_ij,  l_i = sum_j exp(s_ij - m_i),  o_i = sum_j exp(s_ij - m_i) v_j / l_i,
+//   lse_i = m_i + ln l_i
+// over the keys that row i may see; a row that sees none gives o = 0, lse = -inf.  One pass over the keys with a
+// running maximum and sum in f32.  S^T = K Q^T, so a lane owns one query: the row statistics are in-lane plus one
+// exchange of the wave's halves, and P^T, rounded to 16 bits (half a unit in the last place of each weight, the size
+// of the output's own rounding), is at once the B operand of O^T += V^T P^T.  The running maximum is raised only when a
+// tile exceeds it by more than 2^8 (the weights then stay below 2^8, harmless in f32 and in both 16-bit types), which
+// leaves the accumulators alone in nearly all tiles.
+//
+// attn_fwd_kernel: a wave has 32 query rows, a workgroup NW waves that share K / V tiles of 64 keys, double buffered.
+// attn_split_kernel: few rows (single tokens).  All query heads of a key head are rows of one tile, so K / V are read
+// once; each wave walks 32-key tiles of its own (no barrier in the loop), the workgroup's share of the keys is joined in
+// LDS and the shares of several workgroups by attn_join_kernel.
+#include <algorithm>
+#include <cmath>
+
+#include "attention_util.h"
+
+namespace {
+
+// One query tile (32 rows) against key blocks of 32: the state of a wave
+template <int D, bool F16>
+struct FwdState {
+  bf16x8 q[D / 16];
+  f32x16 acc[D / 32];
+  float m, l;      // running maximum (raw scores), sum of this half's weights
+
+  __device__ __forceinline__ void init(const bf16* row, int h) {
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) q[kk] = *reinterpret_cast<const bf16x8*>(row + 16 * kk + 8 * h);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  // NKB blocks of 32 keys; kw[blk] (masked): bit = key of the block this lane's query may see, shifted by 4 h
+  template <int NKB>
+  __device__ __forceinline__ void tile(const TileRead<D>& rd, lds_cptr kt, lds_cptr vt, bool masked, const uint32_t* kw, float c) {
+    f32x16 s[NKB];
+#pragma unroll
+    for (int blk = 0; blk < NKB; ++blk) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[blk][r] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) s[blk] = mfma32x32x16<F16>(rd.row(kt, 32 * blk, kk), q[kk], s[blk]);
+    }
+    if (masked) {
+#pragma unroll
+      for (int blk = 0; blk < NKB; ++blk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[blk][r] = (kw[blk] >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[blk][r] : -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int blk = 0; blk < NKB; ++blk)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[blk][r]);
+    mx = fmaxf(mx, other_half(mx));
+    if (__any(mx > m && !((mx - m) * c <= 8.f))) {
+      const float mn = fmaxf(m, mx);
+      const float a = mn > m ? __builtin_amdgcn_exp2f((m - mn) * c) : 1.f;
+      l *= a;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= a;
+      m = mn;
+    }
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    float t = 0.f;
+#pragma unroll
+    for (int blk = 0; blk < NKB; ++blk)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[blk][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[blk][r], c, -mc));
+        t += s[blk][r];
+      }
+    l += t;
+#pragma unroll
+    for (int blk = 0; blk < NKB; ++blk)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const bf16x8 pf = attn_pack<F16>(s[blk], half);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = mfma32x32x16<F16>(rd.col(vt, 32 * blk + 16 * half, i), pf, acc[i]);
+      }
+  }
+};
+
+template <int D, bool F16, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) attn_fwd_kernel(AttnP p) {
+  constexpr int KT = 64, TB = KT * D * 2;
+  typedef TileStage<D, KT, NW> Stage;
+  __shared__ __attribute__((aligned(1024))) char buf[4 * TB];            // K, V of two tiles
+  __shared__ uint64_t words[ATTN_MASK_KEYS / KT];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int blk = p.nblk - 1 - id % p.nblk, bh = id / p.nblk, b = bh / p.H, hq = bh % p.H, hk = hq / p.G;
+  const int i0 = blk * (32 * NW) + wave * 32;                            // this wave's first row
+  const int row = min(i0 + (lane & 31), p.Lq - 1);
+  const int last = min(blk * (32 * NW) + 32 * NW, p.Lq) - 1;             // the workgroup's last row
+  const int nk = p.causal ? max(0, min(p.Lk, last + p.off + 1)) : p.Lk;
+  const int nt = (nk + KT - 1) / KT;
+
+  FwdState<D, F16> st;
+  st.init(p.q + b * p.sqb + row * p.sql + hq * p.sqh, h);
+  TileRead<D> rd;
+  rd.init(lane);
+  Stage sk, sv;
+  sk.init(lane, wave, p.skl);
+  sv.init(lane, wave, p.svl);
+  const char* kb = uni(p.k + b * p.skb + hk * p.skh);
+  const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  lds_ptr lds = (lds_ptr)buf;
+  LRCE_LDS uint64_t* lw = (LRCE_LDS uint64_t*)words;
+
+  const int chunk = p.mask ? ATTN_MASK_KEYS / KT : nt;
+  for (int c0 = 0; c0 < nt; c0 += chunk) {
+    const int c1 = min(nt, c0 + chunk);
+    if (p.mask) {
+      __syncthreads();
+      attn_pack_mask<NW>(p, b, c0, c1 - c0, lw, lane, wave);
+      __syncthreads();
+    }
+    auto word = [&](int t) { return p.mask ? uni64(lw[t - c0]) : low_bits(p.Lk - t * KT); };
+    auto next = [&](int t, uint64_t& w) {      // the first tile from t on with a visible key
+      for (; t < c1; ++t)
+        if ((w = word(t)) != 0) break;
+      return t;
+    };
+    auto stage = [&](int t, uint64_t w, int cur) {
+      const bool all = w == ~0ull;
+      sk.load(kb + (long long)t * KT * p.skl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + 2 * cur * TB), wave);
+      sv.load(vb + (long long)t * KT * p.svl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + (2 * cur + 1) * TB), wave);
+    };
+    uint64_t w = 0, wn = 0;
+    int t = next(c0, w), cur = 0;
+    if (t < c1) stage(t, w, 0);
+    while (t < c1) {
+      attn_barrier();
+      const int tn = next(t + 1, wn);
+      if (tn < c1) stage(tn, wn, cur ^ 1);
+      const int j0 = t * KT;
+      const int lim = i0 + p.off - j0;                                     // the wave's first row sees keys up to j0 + lim
+      if (!p.causal || lim + 31 >= 0) {
+        const bool diag = p.causal && lim < KT - 1;
+        const bool masked = diag || w != ~0ull;
+        uint32_t kw[2];
+        if (masked) {
+          const int mine = lim + (lane & 31);
+          kw[0] = (uint32_t)w & (diag ? upto(mine) : ~0u);
+          kw[1] = (uint32_t)(w >> 32) & (diag ? upto(mine - 32) : ~0u);
+          kw[0] >>= 4 * h;
+          kw[1] >>= 4 * h;
+        }
+        st.template tile<2>(rd, lds + 2 * cur * TB, lds + (2 * cur + 1) * TB, masked, kw, p.c);
+      }
+      t = tn;
+      w = wn;
+      cur ^= 1;
+    }
+  }
+  const float l = st.l + other_half(st.l);
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const bool valid = i0 + (lane & 31) < p.Lq;
+  bf16* o = p.out + b * p.sob + row * p.sol + hq * p.soh;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) attn_store<F16>(st.acc[i], inv, o + 32 * i, h, valid);
+  if (valid && h == 0) p.lse[(long long)bh * p.Lq + row] = l == 0.f ? -INFINITY : st.m * p.scale + __logf(l);
+}
+
+// The rows of a key head: r = i * G + g for query i and head g of the group, 32 a tile.  A workgroup takes key tiles
+// [split * split_tiles, ...) of 32 keys, wave w every fourth of them.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP p) {
+  constexpr int NW = 4, KT = 32, TB = KT * D * 2, NST = 2;
+  typedef TileStage<D, KT, 1> Stage;
+  constexpr int OP = D + 4;                                              // padded row of a joined output tile (floats)
+  constexpr int SZ = NW * NST * 2 * TB > NW * 32 * OP * 4 ? NW * NST * 2 * TB : NW * 32 * OP * 4;
+  __shared__ __attribute__((aligned(1024))) char buf[SZ];
+  __shared__ uint64_t words[ATTN_MASK_KEYS / 64];
+  __shared__ float sm[NW][32], sl[NW][32];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int sp = id % p.nsplit, rest = id / p.nsplit, rt = rest % p.nblk, bk = rest / p.nblk, b = bk / p.Hk, hk = bk % p.Hk;
+  const int R = p.Lq * p.G;
+  const int r = min(rt * 32 + n, R - 1), qi = r / p.G, hq = hk * p.G + r % p.G;
+  const int last = (min(rt * 32 + 31, R - 1)) / p.G;
+  const int nk = p.causal ? max(0, min(p.Lk, last + p.off + 1)) : p.Lk;
+  const int nt = (nk + KT - 1) / KT;
+  const int b0 = sp * p.split_tiles, b1 = min(nt, b0 + p.split_tiles);   // split_tiles is a multiple of 2
+
+  FwdState<D, F16> st;
+  st.init(p.q + b * p.sqb + qi * p.sql + hq * p.sqh, h);
+  TileRead<D> rd;
+  rd.init(lane);
+  Stage sk, sv;
+  sk.init(lane, 0, p.skl);
+  sv.init(lane, 0, p.svl);
+  const char* kb = uni(p.k + b * p.skb + hk * p.skh);
+  const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  lds_ptr lds = (lds_ptr)buf + wave * (NST * 2 * TB);
+  LRCE_LDS uint64_t* lw = (LRCE_LDS uint64_t*)words;
+
+  const int chunk = p.mask ? ATTN_MASK_KEYS / KT : max(b1 - b0, 1);
+  for (int c0 = b0; c0 < b1; c0 += chunk) {
+    const int c1 = min(b1, c0 + chunk);
+    if (p.mask) {
+      __syncthreads();
+      attn_pack_mask<NW>(p, b, c0 / 2, (c1 - c0 + 1) / 2, lw, lane, wave);
+      __syncthreads();
+    }
+    auto word = [&](int t) {
+      return p.mask ? (uint32_t)(uni64(lw[(t - c0) >> 1]) >> (32 * ((t - c0) & 1))) : (uint32_t)low_bits(p.Lk - t * KT);
+    };
+    auto next = [&](int t, uint32_t& w) {
+      for (; t < c1; t += NW)
+        if ((w = word(t)) != 0) break;
+      return t;
+    };
+    auto stage = [&](int t, uint32_t w, int cur) {
+      const bool all = w == ~0u;
+      sk.load(kb + (long long)t * KT * p.skl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + 2 * cur * TB), 0);
+      sv.load(vb + (long long)t * KT * p.svl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + (2 * cur + 1) * TB), 0);
+    };
+    uint32_t w0 = 0, w1 = 0, w2 = 0;
+    int cur = 0;
+    int t0 = next(c0 + wave, w0);
+    if (t0 < c1) stage(t0, w0, 0);
+    int t1 = next(t0 + NW, w1);
+    if (t1 < c1) stage(t1, w1, 1);
+    while (t0 < c1) {
+      if (t1 < c1) attn_wait_vm<2 * Stage::NI>();
+      else attn_wait_vm<0>();
+      const int lim = p.causal ? qi + p.off - t0 * KT : 31;
+      const bool masked = w0 != ~0u || (p.causal && __any(lim < 31));
+      uint32_t kw[1] = {(w0 & upto(lim)) >> (4 * h)};
+      st.template tile<1>(rd, lds + 2 * cur * TB, lds + (2 * cur + 1) * TB, masked, kw, p.c);
+      const int t2 = next(t1 + NW, w2);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the tile's reads are done: its place may be filled
+      if (t2 < c1) stage(t2, w2, cur);
+      t0 = t1; w0 = w1;
+      t1 = t2; w1 = w2;
+      cur ^= 1;
+    }
+  }
+  // the four waves' shares: o_w relative to m_w, joined at the common maximum
+  const float l = st.l + other_half(st.l);
+  if (h == 0) { sm[wave][n] = st.m; sl[wave][n] = l; }
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(buf) + wave * 32 * OP;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = st.acc[i][4 * u + e];
+      *reinterpret_cast<f32x4*>(so + n * OP + 32 * i + 8 * u + 4 * h) = x;
+    }
+  __syncthreads();
+  constexpr int TPR = 8, DP = D / TPR;                                    // threads a row, values a thread
+  const int rr = threadIdx.x / TPR, part = threadIdx.x % TPR, gr = rt * 32 + rr;
+  if (gr >= R) return;
+  float mx = sm[0][rr];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sm[w][rr]);
+  float ls = 0.f, o[DP];
+#pragma unroll
+  for (int e = 0; e < DP; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const float a = sm[w][rr] == -INFINITY && sl[w][rr] == 0.f ? 0.f : __builtin_amdgcn_exp2f((sm[w][rr] - mx) * p.c);
+    ls += a * sl[w][rr];
+    const float* src = reinterpret_cast<float*>(buf) + (w * 32 + rr) * OP + part * DP;
+#pragma unroll
+    for (int e = 0; e < DP; ++e) o[e] += a == 0.f ? 0.f : a * src[e];
+  }
+  const int gi = gr / p.G, gh = hk * p.G + gr % p.G;
+  const long long grow = ((long long)b * p.H + gh) * p.Lq + gi;
+  if (p.nsplit == 1) {
+    const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+    bf16* dst = p.out + b * p.sob + gi * p.sol + gh * p.soh + part * DP;
+#pragma unroll
+    for (int e = 0; e < DP; e += 4) {
+      bf16x4 x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = to16<F16>(o[e + k] * inv);
+      *reinterpret_cast<bf16x4*>(dst + e) = x;
+    }
+    if (part == 0) p.lse[grow] = ls == 0.f ? -INFINITY : mx * p.scale + __logf(ls);
+  } else {
+    const long long rows = (long long)p.B * p.H * p.Lq;
+    float* dst = p.ws + ((long long)sp * rows + grow) * D + part * DP;
+#pragma unroll
+    for (int e = 0; e < DP; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+    if (part == 0) *reinterpret_cast<float2*>(p.ws2 + 2 * ((long long)sp * rows + grow)) = make_float2(mx, ls);
+  }
+}
+
+// A row's partials of all splits: D / 4 threads a row
+template <int D, bool F16>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnP p) {
+  constexpr int TPR = D / 4;
+  const long long rows = (long long)p.B * p.H * p.Lq;
+  const long long grow = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int part = threadIdx.x % TPR;
+  if (threadIdx.x >= 256 / TPR * TPR || grow >= rows) return;
+  float mx = -INFINITY;
+  for (int s = 0; s < p.nsplit; ++s) mx = fmaxf(mx, p.ws2[2 * (s * rows + grow)]);
+  float ls = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.ws2 + 2 * (s * rows + grow));
+    const float4 x = *reinterpret_cast<const float4*>(p.ws + (s * rows + grow) * D + 4 * part);
+    const float a = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f((ml.x - mx) * p.c);
+    if (a != 0.f || ml.y != ml.y) {
+      ls += a * ml.y;
+      o.x += a * x.x; o.y += a * x.y; o.z += a * x.z; o.w += a * x.w;
+    }
+  }
+  const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+  const int qi = grow % p.Lq, hq = (grow / p.Lq) % p.H;
+  const long long b = grow / p.Lq / p.H;
+  bf16x4 y;
+  y[0] = to16<F16>(o.x * inv); y[1] = to16<F16>(o.y * inv); y[2] = to16<F16>(o.z * inv); y[3] = to16<F16>(o.w * inv);
+  *reinterpret_cast<bf16x4*>(p.out + b * p.sob + qi * p.sol + hq * p.soh + 4 * part) = y;
+  if (part == 0) p.lse[grow] = ls == 0.f ? -INFINITY : mx * p.scale + __logf(ls);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------------- host side
+int attn_check(const LrceAttnDesc* d, const char* what) {
+  if (!d) return lrce_fail(LRCE_E_ARG, "%s: null descriptor", what);
+  if (d->B < 0 || d->H < 1 || d->Hk < 1 || d->Lq < 0 || d->Lk < 0) return lrce_fail(LRCE_E_ARG, "%s: bad sizes B=%d H=%d Hk=%d Lq=%d Lk=%d", what, d->B, d->H, d->Hk, d->Lq, d->Lk);
+  if (d->H % d->Hk) return lrce_fail(LRCE_E_ARG, "%s: %d query heads over %d key heads", what, d->H, d->Hk);
+  if (d->D != 32 && d->D != 64 && d->D != 96 && d->D != 128) return lrce_fail(LRCE_E_ARG, "%s: head dim %d (32, 64, 96 or 128)", what, d->D);
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return lrce_fail(LRCE_E_ARG, "%s: scale must be positive and finite", what);
+  if (d->key_mask && d->mask_bytes != 1 && d->mask_bytes != 4 && d->mask_bytes != 8) return lrce_fail(LRCE_E_ARG, "%s: key mask entries of %d bytes (1, 4 or 8)", what, d->mask_bytes);
+  if (d->B > 0 && d->Lq > 0 && (!d->q || !d->out || !d->lse)) return lrce_fail(LRCE_E_ARG, "%s: null pointer", what);
+  if (d->B > 0 && d->Lk > 0 && (!d->k || !d->v)) return lrce_fail(LRCE_E_ARG, "%s: null pointer", what);
+  const int64_t* st[] = {d->q_stride, d->k_stride, d->v_stride, d->o_stride};
+  const void* at[] = {d->q, d->k, d->v, d->out};
+  for (int i = 0; i < 4; ++i) {
+    if (reinterpret_cast<uintptr_t>(at[i]) % 16) return lrce_fail(LRCE_E_ARG, "%s: tensors must start at multiples of 16 bytes", what);
+    for (int k = 0; k < 3; ++k)
+      if (st[i][k] % 8 || st[i][k] < 0) return lrce_fail(LRCE_E_ARG, "%s: strides must be multiples of 8 elements", what);
+  }
+  // rows are addressed by 32-bit byte offsets inside a tile of 64
+  if (std::max(std::max(d->k_stride[1], d->v_stride[1]), d->q_stride[1]) >= (1ll << 23)) return lrce_fail(LRCE_E_ARG, "%s: a row stride of 2^23 elements or more", what);
+  if ((int64_t)d->Lq + d->Lk >= (1ll << 30)) return lrce_fail(LRCE_E_ARG, "%s: too long", what);
+  if ((int64_t)d->B * d->H * ((d->Lq + 31) / 32) >= (1ll << 31) || (int64_t)d->B * d->H * ((d->Lk + 31) / 32) >= (1ll << 31) ||
+      (int64_t)d->Lq * d->H >= (1ll << 31))
+    return lrce_fail(LRCE_E_ARG, "%s: too many rows", what);
+  return LRCE_OK;
+}
+
+void attn_fill(const LrceAttnDesc* d, AttnP& p) {
+  p = AttnP{};
+  p.q = static_cast<const bf16*>(d->q); p.k = static_cast<const bf16*>(d->k); p.v = static_cast<const bf16*>(d->v);
+  p.out = static_cast<bf16*>(d->out);
+  p.lse = d->lse;
+  p.mask = d->key_mask;
+  p.smb = d->mask_stride; p.mask_bytes = d->mask_bytes;
+  p.sqb = d->q_stride[0]; p.sql = d->q_stride[1]; p.sqh = d->q_stride[2];
+  p.skb = d->k_stride[0]; p.skl = d->k_stride[1]; p.skh = d->k_stride[2];
+  p.svb = d->v_stride[0]; p.svl = d->v_stride[1]; p.svh = d->v_stride[2];
+  p.sob = d->o_stride[0]; p.sol = d->o_stride[1]; p.soh = d->o_stride[2];
+  p.B = d->B; p.H = d->H; p.Hk = d->Hk; p.G = d->H / d->Hk; p.Lq = d->Lq; p.Lk = d->Lk;
+  p.causal = d->causal; p.off = d->Lk - d->Lq;
+  p.scale = d->scale; p.c = d->scale * ATTN_LOG2E;
+  p.dout = static_cast<const bf16*>(d->dout);
+  p.dq = static_cast<bf16*>(d->dq); p.dk = static_cast<bf16*>(d->dk); p.dv = static_cast<bf16*>(d->dv);
+  p.sgb = d->g_stride[0]; p.sgl = d->g_stride[1]; p.sgh = d->g_stride[2];
+  p.dqb = d->dq_stride[0]; p.dql = d->dq_stride[1]; p.dqh = d->dq_stride[2];
+  p.dkb = d->dk_stride[0]; p.dkl = d->dk_stride[1]; p.dkh = d->dk_stride[2];
+  p.dvb = d->dv_stride[0]; p.dvl = d->dv_stride[1]; p.dvh = d->dv_stride[2];
+}
+
+namespace {
+
+struct FwdPlan {
+  bool split;
+  int waves;                 // of a tile-kernel workgroup
+  int nblk, nsplit, split_tiles;
+  int64_t grid, ws;
+};
+
+FwdPlan fwd_plan(const LrceAttnDesc* d) {
+  FwdPlan f{};
+  const int G = d->H / d->Hk;
+  const int64_t rows = (int64_t)d->Lq * G;
+  f.waves = d->Lq <= 64 ? 2 : 4;
+  f.nblk = (d->Lq + 32 * f.waves - 1) / (32 * f.waves);
+  f.grid = (int64_t)d->B * d->H * f.nblk;
+  f.nsplit = 1;
+  f.split = rows <= 32 || (f.grid < 128 && d->Lk >= 1024);
+  if (f.split) {
+    f.nblk = (int)((rows + 31) / 32);
+    const int nt = (d->Lk + 31) / 32;
+    const int64_t base = std::max<int64_t>(1, (int64_t)d->B * d->Hk * f.nblk);
+    const int64_t want = (1024 + base - 1) / base;
+    int n = (int)std::max<int64_t>(1, std::min<int64_t>(want, nt / 8));
+    f.split_tiles = std::max(2, ((nt + n - 1) / n + 1) / 2 * 2);
+    f.nsplit = std::max(1, (nt + f.split_tiles - 1) / f.split_tiles);
+    f.grid = base * f.nsplit;
+    if (f.nsplit > 1) f.ws = (int64_t)f.nsplit * d->B * d->H * d->Lq * (d->D + 2);
+  }
+  return f;
+}
+
+template <int D, bool F16>
+void fwd_launch(const AttnP& p, const FwdPlan& f, hipStream_t s) {
+  if (f.split) {
+    attn_split_kernel<D, F16><<<(unsigned)f.grid, 256, 0, s>>>(p);
+    if (f.nsplit > 1) {
+      const int64_t rows = (int64_t)p.B * p.H * p.Lq, per = 256 / (D / 4);
+      attn_join_kernel<D, F16><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(p);
+    }
+  } else if (f.waves == 2) {
+    attn_fwd_kernel<D, F16, 2><<<(unsigned)f.grid, 128, 0, s>>>(p);
+  } else {
+    attn_fwd_kernel<D, F16, 4><<<(unsigned)f.grid, 256, 0, s>>>(p);
+  }
+}
+
+}  // namespace
+
+extern "C" int64_t lrce_attn_fwd_workspace(const LrceAttnDesc* d) {
+  if (attn_check(d, "attn_fwd_workspace") != LRCE_OK) return -1;
+  return d->B && d->Lq ? fwd_plan(d).ws : 0;
+}
+
+extern "C" int lrce_attn_fwd(const LrceAttnDesc* d, void* stream) {
+  if (const int rc = attn_check(d, "attn_fwd")) return rc;
+  if (d->B == 0 || d->Lq == 0) return LRCE_OK;
+  const FwdPlan f = fwd_plan(d);
+  if (f.grid >= (1ll << 31)) return lrce_fail(LRCE_E_ARG, "attn_fwd: too many rows");
+  if (f.ws && (!d->workspace || d->workspace_elems < f.ws)) return lrce_fail(LRCE_E_ARG, "attn_fwd: a workspace of %lld floats is needed", (long long)f.ws);
+  AttnP p;
+  attn_fill(d, p);
+  p.nblk = f.nblk; p.nsplit = f.nsplit; p.split_tiles = f.split_tiles;
+  p.ws = d->workspace;
+  if (f.ws) p.ws2 = p.ws + (int64_t)f.nsplit * d->B * d->H * d->Lq * d->D;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define LRCE_ATTN_D(N) \
+  case N: \
+    if (d->f16) fwd_launch<N, true>(p, f, s); \
+    else fwd_launch<N, false>(p, f, s); \
+    break;
+  switch (d->D) {
+    LRCE_ATTN_D(32)
+    LRCE_ATTN_D(64)
+    LRCE_ATTN_D(96)
+    LRCE_ATTN_D(128)
+  }
+#undef LRCE_ATTN_D
+  return lrce_check_launch("attn_fwd");
+}

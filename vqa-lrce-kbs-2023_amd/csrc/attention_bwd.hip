@@ -1,0 +1,376 @@
+// Backward of the attention in attention.hip: the weights are recomputed from q, k and the saved log-sum-exp.
+//
+//   p_ij = exp(s_ij - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i   (dk, dv: over the heads that share them)
+//
+// Two kernels, each the only writer of what it sums, so there are no atomics and the result does not depend on timing:
+// attn_dq_kernel has 32 queries a wave and walks the keys (three products; it also leaves lse in base 2 and delta for the
+// other), attn_dkv_kernel has 32 keys a wave and walks the queries of all heads that share them (four products).  The
+// scores are computed twice that way (7 products instead of 5), the price of having no read-modify-write of dq in memory.
+// p and ds are rounded to 16 bits where they become operands; delta and ds are formed in f32.
+#include <algorithm>
+
+#include "attention_util.h"
+
+namespace {
+
+template <int D, bool F16, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
+  constexpr int KT = 64, TB = KT * D * 2;
+  typedef TileStage<D, KT, NW> Stage;
+  __shared__ __attribute__((aligned(1024))) char buf[4 * TB];
+  __shared__ uint64_t words[ATTN_MASK_KEYS / KT];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int blk = p.nblk - 1 - id % p.nblk, bh = id / p.nblk, b = bh / p.H, hq = bh % p.H, hk = hq / p.G;
+  const int i0 = blk * (32 * NW) + wave * 32;
+  const bool valid = i0 + n < p.Lq;
+  const int row = min(i0 + n, p.Lq - 1);
+  const int last = min(blk * (32 * NW) + 32 * NW, p.Lq) - 1;
+  const int nk = p.causal ? max(0, min(p.Lk, last + p.off + 1)) : p.Lk;
+  const int nt = (nk + KT - 1) / KT;
+
+  bf16x8 q[D / 16], g[D / 16];
+  float delta = 0.f;
+  {
+    const bf16* qr = p.q + b * p.sqb + row * p.sql + hq * p.sqh;
+    const bf16* gr = p.dout + b * p.sgb + row * p.sgl + hq * p.sgh;
+    const bf16* orow = p.out + b * p.sob + row * p.sol + hq * p.soh;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      q[kk] = *reinterpret_cast<const bf16x8*>(qr + 16 * kk + 8 * h);
+      g[kk] = *reinterpret_cast<const bf16x8*>(gr + 16 * kk + 8 * h);
+      const bf16x8 o = *reinterpret_cast<const bf16x8*>(orow + 16 * kk + 8 * h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(from16<F16>(g[kk][j]), from16<F16>(o[j]), delta);
+    }
+  }
+  delta += other_half(delta);
+  const float lse = p.lse[(long long)bh * p.Lq + row];
+  // a row that sees no key has lse = -inf and p = exp(s - inf) = 0; so have the rows behind the last
+  const float lse2 = !valid || lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E;
+  const int nst = (p.Lq + 63) / 64 * 2;                                  // 32-row blocks of statistics
+  if (i0 / 32 < nst) p.ws[((long long)bh * nst + i0 / 32) * 64 + lane] = h ? (valid ? delta : 0.f) : lse2;
+
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  TileRead<D> rd;
+  rd.init(lane);
+  Stage sk, sv;
+  sk.init(lane, wave, p.skl);
+  sv.init(lane, wave, p.svl);
+  const char* kb = uni(p.k + b * p.skb + hk * p.skh);
+  const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  lds_ptr lds = (lds_ptr)buf;
+  LRCE_LDS uint64_t* lw = (LRCE_LDS uint64_t*)words;
+  const int chunk = p.mask ? ATTN_MASK_KEYS / KT : nt;
+  for (int c0 = 0; c0 < nt; c0 += chunk) {
+    const int c1 = min(nt, c0 + chunk);
+    if (p.mask) {
+      __syncthreads();
+      attn_pack_mask<NW>(p, b, c0, c1 - c0, lw, lane, wave);
+      __syncthreads();
+    }
+    auto word = [&](int t) { return p.mask ? uni64(lw[t - c0]) : low_bits(p.Lk - t * KT); };
+    auto next = [&](int t, uint64_t& w) {
+      for (; t < c1; ++t)
+        if ((w = word(t)) != 0) break;
+      return t;
+    };
+    auto stage = [&](int t, uint64_t w, int cur) {
+      const bool all = w == ~0ull;
+      sk.load(kb + (long long)t * KT * p.skl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + 2 * cur * TB), wave);
+      sv.load(vb + (long long)t * KT * p.svl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + (2 * cur + 1) * TB), wave);
+    };
+    uint64_t w = 0, wn = 0;
+    int t = next(c0, w), cur = 0;
+    if (t < c1) stage(t, w, 0);
+    while (t < c1) {
+      attn_barrier();
+      const int tn = next(t + 1, wn);
+      if (tn < c1) stage(tn, wn, cur ^ 1);
+      const int lim = i0 + p.off - t * KT;
+      lds_cptr kt = lds + 2 * cur * TB, vt = lds + (2 * cur + 1) * TB;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int ls = lim - 32 * sub;                                   // the wave's first row sees keys up to ls of the block
+        const uint32_t ws = (uint32_t)(w >> (32 * sub));
+        if (ws == 0 || (p.causal && ls + 31 < 0)) continue;
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) s = mfma32x32x16<F16>(rd.row(kt, 32 * sub, kk), q[kk], s);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) dp = mfma32x32x16<F16>(rd.row(vt, 32 * sub, kk), g[kk], dp);
+        const bool diag = p.causal && ls < 31;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -lse2)) * (dp[r] - delta);
+        if (diag || ws != ~0u) {
+          const uint32_t kw = (ws & (diag ? upto(ls + n) : ~0u)) >> (4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = (kw >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : 0.f;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const bf16x8 f = attn_pack<F16>(s, half);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) acc[i] = mfma32x32x16<F16>(rd.col(kt, 32 * sub + 16 * half, i), f, acc[i]);
+        }
+      }
+      t = tn;
+      w = wn;
+      cur ^= 1;
+    }
+  }
+  bf16* o = p.dq + b * p.dqb + row * p.dql + hq * p.dqh;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) attn_store<F16>(acc[i], p.scale, o + 32 * i, h, valid);
+}
+
+// Query tiles of 64 rows (two blocks of 32) of one head at a time; the heads of the group one after the other.  With
+// p.nsplit > 1 a workgroup has its share of the (head, tile) list and leaves f32 sums that attn_dkv_sum_kernel adds in order.
+template <int D, bool F16, int NW>
+__global__ void __launch_bounds__(NW * 64, D <= 96 ? 2 : 1) attn_dkv_kernel(AttnP p) {
+  constexpr int QT = 64, TB = QT * D * 2, SB = 1024;
+  typedef TileStage<D, QT, NW> Stage;
+  __shared__ __attribute__((aligned(1024))) char buf[4 * TB + 2 * SB];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int sp = id % p.nsplit, rest = id / p.nsplit, blk = rest % p.nblk, bk = rest / p.nblk, b = bk / p.Hk, hk = bk % p.Hk;
+  const int j0 = blk * (32 * NW) + wave * 32, jw = blk * (32 * NW);
+  const int j = j0 + n;
+  bool keep = j < p.Lk;
+  if (keep && p.mask) {
+    const long long at = (long long)b * p.smb + j;
+    keep = p.mask_bytes == 1 ? static_cast<const uint8_t*>(p.mask)[at] != 0
+         : p.mask_bytes == 4 ? static_cast<const int*>(p.mask)[at] != 0 : static_cast<const long long*>(p.mask)[at] != 0;
+  }
+  const bool some = __any(keep), allk = __all(keep);
+  const bool work = __syncthreads_or(some);
+
+  bf16x8 kf[D / 16], vf[D / 16];
+  {
+    const long long jr = min(j, p.Lk - 1);
+    const bf16* kr = p.k + b * p.skb + jr * p.skl + hk * p.skh;
+    const bf16* vr = p.v + b * p.svb + jr * p.svl + hk * p.svh;
+    const bf16x8 zero = {};
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      kf[kk] = keep ? *reinterpret_cast<const bf16x8*>(kr + 16 * kk + 8 * h) : zero;
+      vf[kk] = keep ? *reinterpret_cast<const bf16x8*>(vr + 16 * kk + 8 * h) : zero;
+    }
+  }
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { dk[i][r] = 0.f; dv[i][r] = 0.f; }
+
+  TileRead<D> rd;
+  rd.init(lane);
+  Stage sq, sg;
+  sq.init(lane, wave, p.sql);
+  sg.init(lane, wave, p.sgl);
+  lds_ptr lds = (lds_ptr)buf;
+  const int nq = (p.Lq + QT - 1) / QT, nst = nq * 2;
+  const int tf = p.causal ? min(nq, max(0, jw - p.off) / QT) : 0;          // the first tile with a row that sees key jw
+  const int per = nq - tf;
+  const long long total = work ? (long long)p.G * per : 0;
+  const int e0 = (int)(total * sp / p.nsplit), e1 = (int)(total * (sp + 1) / p.nsplit);
+  int hs = per ? e0 / per : 0, ts = tf + (per ? e0 % per : 0);          // the tile being staged
+  auto stage = [&](int cur) {
+    const int hq = hk * p.G + hs;
+    const int rows = p.Lq - ts * QT;
+    const char* qb = uni(p.q + b * p.sqb + hq * p.sqh + (long long)ts * QT * p.sql);
+    const char* gb = uni(p.dout + b * p.sgb + hq * p.sgh + (long long)ts * QT * p.sgl);
+    sq.load(qb, rows, 0, true, attn_lds_u32(lds + 2 * cur * TB), wave);
+    sg.load(gb, rows, 0, true, attn_lds_u32(lds + (2 * cur + 1) * TB), wave);
+    if (wave == 0) attn_glds(uni(p.ws + (((long long)b * p.H + hq) * nst + 2 * ts) * 64), 512, lane * 16, attn_lds_u32(lds + 4 * TB + cur * SB));
+    if (++ts == nq) { ts = tf; ++hs; }
+  };
+  int cur = 0, tc = ts;
+  if (e0 < e1) stage(0);
+  for (int e = e0; e < e1; ++e) {
+    attn_barrier();
+    if (e + 1 < e1) stage(cur ^ 1);
+    lds_cptr qt = lds + 2 * cur * TB, gt = lds + (2 * cur + 1) * TB, stt = lds + 4 * TB + cur * SB;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const int i0 = tc * QT + 32 * sub;
+      const int lim = j0 - p.off - i0;                                   // row i0 + r sees the wave's first key from r = lim on
+      if (!some || i0 >= p.Lq || (p.causal && lim > 31)) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) s = mfma32x32x16<F16>(rd.row(qt, 32 * sub, kk), kf[kk], s);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) dp = mfma32x32x16<F16>(rd.row(gt, 32 * sub, kk), vf[kk], dp);
+      const LRCE_LDS float* sl = (const LRCE_LDS float*)(stt + sub * 256) + 4 * h;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x4 l4 = *reinterpret_cast<const LRCE_LDS f32x4*>(sl + 8 * u);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[4 * u + x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * u + x], p.c, -l4[x]));
+      }
+      if (!allk || (p.causal && lim + 31 > 0)) {
+        const int first = p.causal ? lim + n : -64;                      // rows r >= first see this lane's key
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = keep && crow32(r, h) >= first ? s[r] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x4 d4 = *reinterpret_cast<const LRCE_LDS f32x4*>(sl + 32 + 8 * u);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) dp[4 * u + x] = s[4 * u + x] * (dp[4 * u + x] - d4[x]);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const bf16x8 pf = attn_pack<F16>(s, half), df = attn_pack<F16>(dp, half);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) dv[i] = mfma32x32x16<F16>(rd.col(gt, 32 * sub + 16 * half, i), pf, dv[i]);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) dk[i] = mfma32x32x16<F16>(rd.col(qt, 32 * sub + 16 * half, i), df, dk[i]);
+      }
+    }
+    if (++tc == nq) tc = tf;
+    cur ^= 1;
+  }
+  const bool valid = j < p.Lk;
+  if (p.nsplit == 1) {
+    bf16* ok = p.dk + b * p.dkb + (long long)j * p.dkl + hk * p.dkh;
+    bf16* ov = p.dv + b * p.dvb + (long long)j * p.dvl + hk * p.dvh;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      attn_store<F16>(dk[i], p.scale, ok + 32 * i, h, valid);
+      attn_store<F16>(dv[i], 1.f, ov + 32 * i, h, valid);
+    }
+  } else if (valid) {
+    // [split][dk, dv][B Hk Lk][D]
+    const long long rows = (long long)p.B * p.Hk * p.Lk, at = (long long)bk * p.Lk + j;
+    float* wk = p.ws2 + (2ll * sp * rows + at) * D;
+    float* wv = wk + rows * D;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        f32x4 x, y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[e] = dk[i][4 * u + e] * p.scale; y[e] = dv[i][4 * u + e]; }
+        *reinterpret_cast<f32x4*>(wk + 32 * i + 8 * u + 4 * h) = x;
+        *reinterpret_cast<f32x4*>(wv + 32 * i + 8 * u + 4 * h) = y;
+      }
+  }
+}
+
+// dk / dv rows: the splits' f32 sums in order, one rounding.  A thread has 4 values.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256) attn_dkv_sum_kernel(AttnP p) {
+  const long long rows = (long long)p.B * p.Hk * p.Lk, n = 2 * rows * (D / 4);
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(p.ws2 + 2ll * s * rows * D + 4 * e);
+    a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+  }
+  const int part = e % (D / 4);
+  const long long at = e / (D / 4) % rows, j = at % p.Lk, bk = at / p.Lk, b = bk / p.Hk, hk = bk % p.Hk;
+  bf16* dst = e >= rows * (D / 4) ? p.dv + b * p.dvb + j * p.dvl + hk * p.dvh : p.dk + b * p.dkb + j * p.dkl + hk * p.dkh;
+  bf16x4 y;
+  y[0] = to16<F16>(a.x); y[1] = to16<F16>(a.y); y[2] = to16<F16>(a.z); y[3] = to16<F16>(a.w);
+  *reinterpret_cast<bf16x4*>(dst + 4 * part) = y;
+}
+
+struct BwdPlan {
+  int wq, wk, nbq, nbk, nsplit;
+  int64_t gq, gk, stat, part;
+};
+
+BwdPlan bwd_plan(const LrceAttnDesc* d) {
+  BwdPlan f{};
+  f.wq = d->Lq <= 64 ? 2 : 4;
+  f.wk = d->Lk <= 64 ? 2 : 4;
+  f.nbq = (d->Lq + 32 * f.wq - 1) / (32 * f.wq);
+  f.nbk = (d->Lk + 32 * f.wk - 1) / (32 * f.wk);
+  f.gq = (int64_t)d->B * d->H * f.nbq;
+  f.stat = (int64_t)d->B * d->H * ((d->Lq + 63) / 64) * 128;
+  const int64_t base = std::max<int64_t>(1, (int64_t)d->B * d->Hk * f.nbk), tiles = (int64_t)(d->H / d->Hk) * ((d->Lq + 63) / 64);
+  f.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((768 + base - 1) / base, tiles / 8));
+  f.gk = (int64_t)d->B * d->Hk * f.nbk * f.nsplit;
+  if (f.nsplit > 1) f.part = 2ll * f.nsplit * d->B * d->Hk * d->Lk * d->D;
+  return f;
+}
+
+template <int D, bool F16>
+void bwd_launch(AttnP p, const BwdPlan& f, hipStream_t s) {
+  if (f.gq) {
+    p.nblk = f.nbq;
+    if (f.wq == 2) attn_dq_kernel<D, F16, 2><<<(unsigned)f.gq, 128, 0, s>>>(p);
+    else attn_dq_kernel<D, F16, 4><<<(unsigned)f.gq, 256, 0, s>>>(p);
+  }
+  if (f.gk) {
+    p.nblk = f.nbk;
+    p.nsplit = f.nsplit;
+    if (f.wk == 2) attn_dkv_kernel<D, F16, 2><<<(unsigned)f.gk, 128, 0, s>>>(p);
+    else attn_dkv_kernel<D, F16, 4><<<(unsigned)f.gk, 256, 0, s>>>(p);
+    if (f.nsplit > 1) {
+      const int64_t n = 2ll * p.B * p.Hk * p.Lk * (D / 4);
+      attn_dkv_sum_kernel<D, F16><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
+    }
+  }
+}
+
+int bwd_check(const LrceAttnDesc* d, const char* what) {
+  if (const int rc = attn_check(d, what)) return rc;
+  const int64_t* st[] = {d->g_stride, d->dq_stride, d->dk_stride, d->dv_stride};
+  const void* at[] = {d->dout, d->dq, d->dk, d->dv};
+  for (int i = 0; i < 4; ++i) {
+    if (d->B > 0 && (i < 2 ? d->Lq : d->Lk) > 0 && !at[i]) return lrce_fail(LRCE_E_ARG, "%s: null gradient pointer", what);
+    if (reinterpret_cast<uintptr_t>(at[i]) % 16) return lrce_fail(LRCE_E_ARG, "%s: tensors must start at multiples of 16 bytes", what);
+    for (int k = 0; k < 3; ++k)
+      if (st[i][k] % 8 || st[i][k] < 0) return lrce_fail(LRCE_E_ARG, "%s: strides must be multiples of 8 elements", what);
+  }
+  if (d->g_stride[1] >= (1ll << 23)) return lrce_fail(LRCE_E_ARG, "%s: a row stride of 2^23 elements or more", what);
+  return LRCE_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t lrce_attn_bwd_workspace(const LrceAttnDesc* d) {
+  if (attn_check(d, "attn_bwd_workspace") != LRCE_OK) return -1;
+  const BwdPlan f = bwd_plan(d);
+  return f.stat + f.part;
+}
+
+extern "C" int lrce_attn_bwd(const LrceAttnDesc* d, void* stream) {
+  if (const int rc = bwd_check(d, "attn_bwd")) return rc;
+  if (d->B == 0) return LRCE_OK;
+  const BwdPlan f = bwd_plan(d);
+  if (f.gq >= (1ll << 31) || f.gk >= (1ll << 31) || (int64_t)d->B * d->Hk * d->Lk * (d->D / 2) >= (1ll << 38))
+    return lrce_fail(LRCE_E_ARG, "attn_bwd: too many rows");
+  if (f.stat + f.part && (!d->workspace || d->workspace_elems < f.stat + f.part))
+    return lrce_fail(LRCE_E_ARG, "attn_bwd: a workspace of %lld floats is needed", (long long)(f.stat + f.part));
+  AttnP p;
+  attn_fill(d, p);
+  p.ws = d->workspace;
+  p.ws2 = p.ws + f.stat;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define LRCE_ATTN_D(N) \
+  case N: \
+    if (d->f16) bwd_launch<N, true>(p, f, s); \
+    else bwd_launch<N, false>(p, f, s); \
+    break;
+  switch (d->D) {
+    LRCE_ATTN_D(32)
+    LRCE_ATTN_D(64)
+    LRCE_ATTN_D(96)
+    LRCE_ATTN_D(128)
+  }
+#undef LRCE_ATTN_D
+  return lrce_check_launch("attn_bwd");
+}

@@ -1,0 +1,208 @@
+// Device helpers shared by the attention kernels (attention.hip: forward; attention_bwd.hip: backward).
+// Internal linkage: included by each .hip.
+//
+// Layout facts that all of them use (wave64, v_mfma_f32_32x32x16):
+//  * an accumulator tile [m][n] holds n = lane & 31 and m = (reg & 3) + 8 (reg >> 2) + 4 (lane >> 5);
+//  * its registers 8s .. 8s+7, rounded to 16 bits, are a B operand [k][n] whose k runs over the 16 rows of
+//    slice s in the order 4h + {0..3}, 8 + 4h + {0..3} (h = lane >> 5).  The contraction does not care about
+//    the order as long as the A operand follows it, so a score tile feeds the next product from registers;
+//  * that A operand is the transpose of a row-major tile: ds_read_b64_tr_b16 delivers it from LDS.
+// Tiles lie in LDS row-major, 2 D bytes a row, their 16-byte chunks XOR-swizzled by a function of the row
+// under which both the row reads (8 rows, one chunk) and the transposing reads (4 rows, a chunk pair) fall on
+// all banks.  They are filled by buffer loads straight to LDS: rows past the end or masked out are given an
+// offset outside the buffer and arrive as zeros, so what memory holds there (NaN included) enters no product.
+#pragma once
+#include "common.h"
+#include "lrce_capi.h"
+
+// kernel arguments
+struct AttnP {
+  const bf16 *q, *k, *v, *dout;
+  bf16 *out, *dq, *dk, *dv;
+  float* lse;          // [B][H][Lq]
+  const void* mask;    // [B][Lk], mask_bytes an entry, 0 = key hidden
+  long long sqb, sql, sqh, skb, skl, skh, svb, svl, svh, sob, sol, soh, sgb, sgl, sgh;   // strides of q, k, v, out, dout
+  long long dqb, dql, dqh, dkb, dkl, dkh, dvb, dvl, dvh;                                   // of dq, dk, dv
+  long long smb;
+  int B, H, Hk, G, Lq, Lk, causal, mask_bytes, off;   // G = H / Hk, off = Lk - Lq
+  float scale, c;      // c = scale * log2(e)
+  int nblk, nsplit, split_tiles;
+  float* ws;           // forward: partials of the splits; backward: row statistics, then partials
+  float* ws2;
+};
+
+// host side, shared by the two files' entry points: argument checks (an LRCE_E_* code) and the kernel arguments
+int attn_check(const LrceAttnDesc* d, const char* what);
+void attn_fill(const LrceAttnDesc* d, AttnP& p);
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef LRCE_LDS char* lds_ptr;
+typedef const LRCE_LDS char* lds_cptr;
+
+constexpr float ATTN_LOG2E = 1.4426950408889634f;
+constexpr int ATTN_MASK_KEYS = 16384;   // keys whose mask bits lie in LDS at a time
+
+__device__ __forceinline__ int crow32(int reg, int h) { return (reg & 3) + 8 * (reg >> 2) + 4 * h; }
+
+// XOR of the 16-byte chunk index: 3 bits where a row has 8 or 16 chunks, 2 bits where it has 4 or 12
+template <int D>
+__device__ __forceinline__ int attn_swz(int row) {
+  if constexpr (D % 64 == 0) return ((row & 3) << 1) | ((row >> 2) & 1);
+  else return (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
+}
+
+// Per-lane byte offsets of the operand reads of a tile [rows][D]
+template <int D>
+struct TileRead {
+  static constexpr int NV = D % 64 == 0 ? 4 : 2, NT = D % 64 == 0 ? 2 : 1, PITCH = 2 * D;
+  int ka[NV], va[NT];
+  __device__ __forceinline__ void init(int lane) {
+    const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) ka[j] = r * PITCH + (((2 * j + h) ^ attn_swz<D>(r)) << 4);
+    const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3, row = 4 * (g >> 1) + q;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      va[j] = row * PITCH + (((4 * j + 2 * (g & 1) + (p >> 1)) ^ attn_swz<D>(row)) << 4) + (p & 1) * 8;
+  }
+  // A[m = row r0 + lane & 31][k = 16 kk + 8 h ..]   (r0 a multiple of 32)
+  __device__ __forceinline__ bf16x8 row(lds_cptr t, int r0, int kk) const {
+    return *reinterpret_cast<const LRCE_LDS bf16x8*>(t + ka[kk % NV] + (kk / NV) * (NV * 32) + r0 * PITCH);
+  }
+  // A[m = column 32 blk + lane & 31][k = rows r0 .. r0 + 15 in the accumulator's order]   (r0 a multiple of 16)
+  __device__ __forceinline__ bf16x8 col(lds_cptr t, int r0, int blk) const {
+    bf16x8 o;
+#pragma unroll
+    for (int h2 = 0; h2 < 2; ++h2) {
+      lds_cptr a = t + va[blk % NT] + (blk / NT) * (NT * 64) + (r0 + 8 * h2) * PITCH;
+      s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LRCE_LDS s16x4*)(a));
+      const bf16x4 b = __builtin_bit_cast(bf16x4, v);
+      o[4 * h2 + 0] = b[0]; o[4 * h2 + 1] = b[1]; o[4 * h2 + 2] = b[2]; o[4 * h2 + 3] = b[3];
+    }
+    return o;
+  }
+};
+
+__device__ __forceinline__ uint32_t attn_lds_u32(lds_cptr p) { return (uint32_t)(uintptr_t)p; }
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const char* uni(const void* p) {
+  const uint64_t a = reinterpret_cast<uintptr_t>(p);
+  return reinterpret_cast<const char*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a) |
+                                       ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32));
+}
+
+// 64 lanes x 16 bytes from base + voff (zeros where voff + 16 > bytes) to LDS at dst (wave-uniform, 1 KB).  In asm, so
+// that the compiler does not drain the loads in flight before every LDS read; the loops' own waits order them.
+__device__ __forceinline__ void attn_glds(const char* base, uint32_t bytes, uint32_t voff, uint32_t dst) {
+  const uint64_t a = reinterpret_cast<uintptr_t>(base);
+  i32x4 rs;
+  rs[0] = (int)(uint32_t)a;
+  rs[1] = (int)(uint32_t)((a >> 32) & 0xffffu);
+  rs[2] = (int)bytes;
+  rs[3] = 0x00020000;
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(voff), "s"(rs), "s"(dst) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void attn_wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// this wave's loads have landed and every wave is past its reads
+__device__ __forceinline__ void attn_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Staging of a tile [ROWS][D] by NW waves: NI loads of 1 KB each a wave
+template <int D, int ROWS, int NW>
+struct TileStage {
+  static constexpr int CH = D / 8, NI = ROWS * CH / (64 * NW), BYTES = ROWS * D * 2;
+  static_assert(NI * 64 * NW == ROWS * CH, "whole loads");
+  uint32_t voff[NI];
+  int rowi[NI];
+  uint32_t pitch;
+  __device__ __forceinline__ void init(int lane, int wave, long long ld) {
+    pitch = (uint32_t)(ld * 2);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int id = (i * NW + wave) * 64 + lane, row = id / CH, cp = id % CH;
+      rowi[i] = row;
+      voff[i] = (uint32_t)row * pitch + (uint32_t)((cp ^ attn_swz<D>(row)) << 4);
+    }
+  }
+  // rows [0, n) of the tile at base (0 < n); keep: bit r = 0 leaves row r zero
+  __device__ __forceinline__ void load(const char* base, int n, uint64_t keep, bool all, uint32_t dst, int wave) const {
+    const uint32_t bytes = (uint32_t)(min(n, ROWS) - 1) * pitch + 2 * D;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      uint32_t o = voff[i];
+      if (!all) o = ((keep >> rowi[i]) & 1) ? o : 0x80000000u;
+      attn_glds(base, bytes, o, dst + (uint32_t)(i * NW + wave) * 1024);
+    }
+  }
+};
+
+// Mask bits of the 64-key tiles [t0, t0 + n) of batch row b: bit j of word w = key 64 (t0 + w) + j is there and not hidden
+template <int NW>
+__device__ __forceinline__ void attn_pack_mask(const AttnP& p, int b, int t0, int n, LRCE_LDS uint64_t* words, int lane, int wave) {
+  for (int w = wave; w < n; w += NW) {
+    const int j = (t0 + w) * 64 + lane;
+    bool on = j < p.Lk;
+    if (on) {
+      const long long at = (long long)b * p.smb + j;
+      on = p.mask_bytes == 1 ? static_cast<const uint8_t*>(p.mask)[at] != 0
+         : p.mask_bytes == 4 ? static_cast<const int*>(p.mask)[at] != 0 : static_cast<const long long*>(p.mask)[at] != 0;
+    }
+    const uint64_t bits = __ballot(on);
+    if (lane == 0) words[w] = bits;
+  }
+}
+__device__ __forceinline__ uint64_t uni64(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x) |
+         ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32);
+}
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+// the low n + 1 bits of a word (n < 0: none)
+__device__ __forceinline__ uint32_t upto(int n) { return n >= 31 ? ~0u : n < 0 ? 0u : (2u << n) - 1; }
+
+__device__ __forceinline__ float other_half(float x) {
+  const unsigned u = __float_as_uint(x);
+  const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? s[0] : s[1]);
+}
+
+// registers 8s .. 8s+7 of an accumulator tile as 16-bit values (round to nearest)
+template <bool F16>
+__device__ __forceinline__ bf16x8 attn_pack(const f32x16& a, int s) {
+  bf16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = to16<F16>(a[8 * s + j]);
+  return o;
+}
+
+// A transposed accumulator tile [d = 32 rows][row = lane & 31], times mul, into the row at dst (16 bits): the halves
+// exchange 4-value groups so that each lane stores 16 bytes at a time
+template <bool F16>
+__device__ __forceinline__ void attn_store(const f32x16& a, float mul, bf16* dst, int h, bool valid) {
+#pragma unroll
+  for (int u = 0; u < 4; u += 2) {
+    unsigned x[2], y[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      bf16x2 t;
+      t[0] = to16<F16>(a[4 * u + 2 * e] * mul); t[1] = to16<F16>(a[4 * u + 2 * e + 1] * mul);
+      x[e] = __builtin_bit_cast(unsigned, t);
+      t[0] = to16<F16>(a[4 * u + 4 + 2 * e] * mul); t[1] = to16<F16>(a[4 * u + 5 + 2 * e] * mul);
+      y[e] = __builtin_bit_cast(unsigned, t);
+    }
+    uint4 o;
+    const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+    const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+    o.x = s0[0]; o.y = s1[0]; o.z = s0[1]; o.w = s1[1];
+    if (valid) *reinterpret_cast<uint4*>(dst + 8 * (u + h)) = o;
+  }
+}
+
+}  // namespace

@@ -76,6 +76,15 @@ class MhaDesc(ctypes.Structure):
     ]
 
 
+class AttnDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "key_mask")]
+                + [(f"{n}_s{a}", ctypes.c_int64) for n in "qkvo" for a in "blh"] + [("mask_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("B", "H", "Hk", "Lq", "Lk", "D", "f16", "causal", "mask_bytes")]
+                + [("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_elems", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("dout", "dq", "dk", "dv")]
+                + [(f"{n}_s{a}", ctypes.c_int64) for n in ("g", "dq", "dk", "dv") for a in "blh"])
+
+
 class LnPrologue(ctypes.Structure):
     _fields_ = [
         ("mode", ctypes.c_int32), ("gamma", ctypes.c_void_p), ("beta", ctypes.c_void_p), ("eps", ctypes.c_float),
@@ -210,6 +219,10 @@ _SIGS = {
     "lrce_layernorm_bwd_f16s_deferred": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _F, _U64, _P, _I64, _P, _P],
     "lrce_mha_fwd": [ctypes.POINTER(MhaDesc), _P],
     "lrce_mha_bwd": [ctypes.POINTER(MhaDesc), _P],
+    "lrce_attn_fwd": [ctypes.POINTER(AttnDesc), _P],
+    "lrce_attn_bwd": [ctypes.POINTER(AttnDesc), _P],
+    "lrce_attn_fwd_workspace": [ctypes.POINTER(AttnDesc)],
+    "lrce_attn_bwd_workspace": [ctypes.POINTER(AttnDesc)],
     "lrce_dec_sa_fwd": [ctypes.POINTER(DecSa), _P],
     "lrce_dec_ca_fwd": [ctypes.POINTER(DecCa), _P],
     "lrce_dec_ca_bwd": [ctypes.POINTER(DecCaBwd), _P],
@@ -260,6 +273,7 @@ _RET["lrce_dec_slab_elems"] = _I64
 _SIGS["lrce_wattn_dbias_part_elems"] = [_I, _I, _I]
 _RET.update({"lrce_dec_step_field": _I64, "lrce_dec_step_ws_elems": _I64, "lrce_dec_step_counter_words": _I64})
 _SIGS["lrce_layernorm_bwd_workspace"] = [_I, _I]
+_RET.update({"lrce_attn_fwd_workspace": _I64, "lrce_attn_bwd_workspace": _I64})
 
 
 def _declare(L):

@@ -653,6 +653,114 @@ def mha_desc(q, Lq, *, k1, v1, lk1, ld_kv1, stride_kv1_b, kv1_bdiv=1, k2=None, v
     return m
 
 
+# ---- attention at general lengths (csrc/attention.hip, attention_bwd.hip) ---------------------------
+_MASK_BYTES = {torch.bool: 1, torch.uint8: 1, torch.int8: 1, torch.int32: 4, torch.int64: 8}
+
+
+def _call_on(name, t, *args):
+    """N.call with t's device as the current one: a launch goes to the device of its stream."""
+    if t.device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(t.device):
+        return call(name, *args)
+
+
+def _strides(t):
+    """Strides of all but the last axis; 0 for an axis of length 1, whose stride says nothing."""
+    return [st if n > 1 else 0 for st, n in zip(t.stride()[:-1], t.shape[:-1])]
+
+
+def _rows16(t):
+    """t, or a contiguous copy where its rows are not whole 16-byte pieces as the kernels read them."""
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and not any(
+            s % 8 or s >= 1 << 23 for s in _strides(t)[1:]) and _strides(t)[0] % 8 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _attn_args(what, q, k, v, key_mask, causal, scale):
+    """Checked (q, k, v, mask, scale) of the attention operators."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _chk(t, q.dtype, f"{what}: {name}")
+        if t.device != q.device:
+            raise N.NativeError(f"{what}: {name} is on {t.device}, q on {q.device}")
+        if t.dim() != 4:
+            raise N.NativeError(f"{what}: {name} must be [batch, length, heads, head dim], got {tuple(t.shape)}")
+    if q.dtype not in (BF16, F16):
+        raise N.NativeError(f"{what}: bf16 or fp16, got {q.dtype}")
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hk < 1 or H < 1 or H % Hk:
+        raise N.NativeError(f"{what}: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if D not in (32, 64, 96, 128):
+        raise N.NativeError(f"{what}: head dim {D} (32, 64, 96 or 128)")
+    if key_mask is not None:
+        if not key_mask.is_cuda or key_mask.device != q.device or key_mask.dtype not in _MASK_BYTES:
+            raise N.NativeError(f"{what}: key_mask must be bool or integer on {q.device}")
+        if key_mask.shape != (B, Lk):
+            raise N.NativeError(f"{what}: key_mask must be {(B, Lk)}, got {tuple(key_mask.shape)}")
+        if Lk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise N.NativeError(f"{what}: scale must be positive and finite, got {scale}")
+    return _rows16(q), _rows16(k), _rows16(v), key_mask, scale
+
+
+def _attn_desc(q, k, v, out, lse, key_mask, causal, scale, dout=None, dq=None, dk=None, dv=None):
+    B, Lq, H, D = q.shape
+    m = key_mask
+    grads = (dout, dq, dk, dv)
+    return N.AttnDesc(ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(m), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
+                      0 if m is None or B <= 1 else m.stride(0), B, H, k.shape[2], Lq, k.shape[1], D, q.dtype == F16, bool(causal),
+                      0 if m is None else _MASK_BYTES[m.dtype], scale, None, 0, *(ptr(t) for t in grads),
+                      *(s for t in grads for s in (_strides(t) if t is not None else (0, 0, 0))))
+
+
+def attention(q, k, v, key_mask=None, causal=False, scale=None):
+    """Multi-head attention: (out [B, Lq, H, D], lse f32 [B, H, Lq]) of q [B, Lq, H, D] and k, v [B, Lk, Hk, D] (bf16 or fp16,
+    D 32 / 64 / 96 / 128, H a multiple of Hk: query head h reads key head h // (H // Hk); any batch / row / head strides).
+    key_mask [B, Lk] (bool or integer, 0 = hidden); causal: row i sees the keys j <= i + Lk - Lq; scale (positive): D ** -0.5 by
+    default.  A row that sees no key gives 0 and lse -inf.  k and v may hold anything at keys that key_mask hides; at keys
+    that only causality hides they must be finite.  lse is the natural logarithm of the row's sum, for attention_bwd."""
+    q, k, v, key_mask, scale = _attn_args("attention", q, k, v, key_mask, causal, scale)
+    B, Lq, H, D = q.shape
+    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Lq), dtype=F32, device=q.device)
+    d = _attn_desc(q, k, v, out, lse, key_mask, causal, scale)
+    n = N.lib().lrce_attn_fwd_workspace(ctypes.byref(d))
+    if n > 0:
+        ws = torch.empty(n, dtype=F32, device=q.device)
+        d.workspace, d.workspace_elems = ptr(ws), n
+    _call_on("lrce_attn_fwd", q, ctypes.byref(d), stream_of(q))
+    return out, lse
+
+
+def attention_bwd(dout, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
+    """(dq, dk, dv) of attention() for dout, with the forward's out and lse; the arguments as there.  Sums over the query
+    heads that share a key head are formed in f32; the result does not depend on timing."""
+    q, k, v, key_mask, scale = _attn_args("attention_bwd", q, k, v, key_mask, causal, scale)
+    B, Lq, H, D = q.shape
+    for name, t in (("dout", dout), ("out", out)):
+        _chk(t, q.dtype, f"attention_bwd: {name}")
+        if t.shape != q.shape or t.device != q.device:
+            raise N.NativeError(f"attention_bwd: {name} must be {tuple(q.shape)} on {q.device}, got {tuple(t.shape)} on {t.device}")
+    _chk(lse, F32, "attention_bwd: lse")
+    if lse.shape != (B, H, Lq) or lse.device != q.device:
+        raise N.NativeError(f"attention_bwd: lse must be {(B, H, Lq)} on {q.device}, got {tuple(lse.shape)} on {lse.device}")
+    dout, out, lse = _rows16(dout), _rows16(out), lse.contiguous()
+    dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    d = _attn_desc(q, k, v, out, lse, key_mask, causal, scale, dout, dq, dk, dv)
+    n = N.lib().lrce_attn_bwd_workspace(ctypes.byref(d))
+    if n > 0:
+        ws = torch.empty(n, dtype=F32, device=q.device)
+        d.workspace, d.workspace_elems = ptr(ws), n
+    _call_on("lrce_attn_bwd", q, ctypes.byref(d), stream_of(q))
+    return dq, dk, dv
+
+
 # ---- recurrent decoder: per-head fused attention blocks (csrc/decoder.hip) -------------------------
 DEC_MAX_ROWS = 64
 _DEC_WS = {}
