@@ -400,6 +400,42 @@ int64_t lrce_attn_bwd_workspace(const LrceAttnDesc* desc);
 int lrce_attn_fwd(const LrceAttnDesc* desc, void* stream);
 int lrce_attn_bwd(const LrceAttnDesc* desc, void* stream);
 
+/* Per-head RMS norm of queries and keys with the rotary position embedding in the same pass: q [B][L][H][D], k [B][L][Hk][D]
+ * (dtype 0 bf16, 1 fp16, 2 f32; D a multiple of 8 up to 256), strides (batch, row, head) in elements, the last axis
+ * contiguous.  y = rotate(x rsqrt(mean(x^2) + eps) w): the first R of D dims (even) as pairs (i, R/2 + i), or (2i, 2i + 1)
+ * with interleaved, by the angle position * inv_freq[i] (formed in 64 bits); positions [B][L] int32 / int64 (pos_bytes 4 / 8,
+ * batch stride pos_stride, rows contiguous).  Backward: q_out / k_out = dq / dk from gq / gk (gradients of the outputs), and
+ * the weights' gradients dq_weight / dk_weight (f32 [D], stored); lrce_qk_norm_rope_bwd_workspace() floats. */
+typedef struct LrceRopeDesc {
+  const void *q, *k;
+  const float *q_weight, *k_weight;
+  const void* positions;
+  const float* inv_freq;
+  void *q_out, *k_out;
+  const void *gq, *gk;
+  float *dq_weight, *dk_weight;
+  float* workspace;
+  int64_t workspace_elems;
+  int64_t q_stride[3], k_stride[3], qo_stride[3], ko_stride[3], gq_stride[3], gk_stride[3];
+  int64_t pos_stride;
+  int32_t B, L, H, Hk, D, R, dtype, interleaved, pos_bytes;
+  float eps;
+} LrceRopeDesc;
+
+int lrce_qk_norm_rope_fwd(const LrceRopeDesc* desc, void* stream);
+int64_t lrce_qk_norm_rope_bwd_workspace(const LrceRopeDesc* desc);
+int lrce_qk_norm_rope_bwd(const LrceRopeDesc* desc, void* stream);
+
+/* Embedding lookup y[i][:] = scale * w[ids[i]][:] (types 0 bf16, 1 fp16, 2 f32; y has w's type, or any where w is f32; ids int32 /
+ * int64 (ids_bytes 4 / 8); an id outside [0, rows) gives a row of NaN) and its gradient dw[v][:] (f32 [rows][cols], contiguous)
+ * = (accumulate: +=) scale * sum over ids[i] = v of dy[i][:], in token order (tokens sorted by id, no atomics on the sums: the
+ * same bits each time); ids outside the table and padding_idx (-1: none) have no gradient. */
+int lrce_embedding_fwd(const void* ids, int ids_bytes, int64_t n, const void* w, int64_t ld_w, int64_t rows, int cols, int w_type,
+                       void* y, int y_type, float scale, void* stream);
+int64_t lrce_embedding_bwd_workspace(int64_t n, int64_t rows, int cols);
+int lrce_embedding_bwd(const void* ids, int ids_bytes, int64_t n, const void* dy, int dy_type, float* dw, int64_t rows, int cols,
+                       float scale, int64_t padding_idx, int accumulate, float* workspace, int64_t workspace_elems, void* stream);
+
 /* ---------------------------------------------------------------- recurrent decoder attention blocks
  * One nn.TransformerDecoderLayer (fusionv3.py:8-17: d_model 768, 12 heads x 64, post-norm, one query
  * token per row) has two attention blocks that factor by head; each is ONE launch of B x 12

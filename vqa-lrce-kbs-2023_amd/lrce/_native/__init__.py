@@ -85,6 +85,16 @@ class AttnDesc(ctypes.Structure):
                 + [(f"{n}_s{a}", ctypes.c_int64) for n in ("g", "dq", "dk", "dv") for a in "blh"])
 
 
+class RopeDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "q_weight", "k_weight", "positions", "inv_freq", "q_out", "k_out", "gq", "gk",
+                                                "dq_weight", "dk_weight", "workspace")]
+                + [("workspace_elems", ctypes.c_int64)]
+                + [(f"{n}_s{a}", ctypes.c_int64) for n in ("q", "k", "qo", "ko", "gq", "gk") for a in "blh"]
+                + [("pos_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("B", "L", "H", "Hk", "D", "R", "dtype", "interleaved", "pos_bytes")]
+                + [("eps", ctypes.c_float)])
+
+
 class LnPrologue(ctypes.Structure):
     _fields_ = [
         ("mode", ctypes.c_int32), ("gamma", ctypes.c_void_p), ("beta", ctypes.c_void_p), ("eps", ctypes.c_float),
@@ -223,6 +233,12 @@ _SIGS = {
     "lrce_attn_bwd": [ctypes.POINTER(AttnDesc), _P],
     "lrce_attn_fwd_workspace": [ctypes.POINTER(AttnDesc)],
     "lrce_attn_bwd_workspace": [ctypes.POINTER(AttnDesc)],
+    "lrce_qk_norm_rope_fwd": [ctypes.POINTER(RopeDesc), _P],
+    "lrce_qk_norm_rope_bwd": [ctypes.POINTER(RopeDesc), _P],
+    "lrce_qk_norm_rope_bwd_workspace": [ctypes.POINTER(RopeDesc)],
+    "lrce_embedding_fwd": [_P, _I, _I64, _P, _I64, _I64, _I, _I, _P, _I, _F, _P],
+    "lrce_embedding_bwd_workspace": [_I64, _I64, _I],
+    "lrce_embedding_bwd": [_P, _I, _I64, _P, _I, _P, _I64, _I, _F, _I64, _I, _P, _I64, _P],
     "lrce_dec_sa_fwd": [ctypes.POINTER(DecSa), _P],
     "lrce_dec_ca_fwd": [ctypes.POINTER(DecCa), _P],
     "lrce_dec_ca_bwd": [ctypes.POINTER(DecCaBwd), _P],
@@ -273,7 +289,8 @@ _RET["lrce_dec_slab_elems"] = _I64
 _SIGS["lrce_wattn_dbias_part_elems"] = [_I, _I, _I]
 _RET.update({"lrce_dec_step_field": _I64, "lrce_dec_step_ws_elems": _I64, "lrce_dec_step_counter_words": _I64})
 _SIGS["lrce_layernorm_bwd_workspace"] = [_I, _I]
-_RET.update({"lrce_attn_fwd_workspace": _I64, "lrce_attn_bwd_workspace": _I64})
+_RET.update({n: _I64 for n in ("lrce_attn_fwd_workspace", "lrce_attn_bwd_workspace", "lrce_qk_norm_rope_bwd_workspace",
+                               "lrce_embedding_bwd_workspace")})
 
 
 def _declare(L):

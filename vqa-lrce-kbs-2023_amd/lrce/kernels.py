@@ -761,6 +761,143 @@ def attention_bwd(dout, q, k, v, out, lse, key_mask=None, causal=False, scale=No
     return dq, dk, dv
 
 
+# ---- query / key norm with the position rotation (csrc/qk_rope.hip) ---------------------------------
+_TYPE = {BF16: 0, F16: 1, F32: 2}
+_INT_BYTES = {torch.int32: 4, torch.int64: 8}
+
+
+def _rope_args(what, q, k, q_weight, k_weight, positions, inv_freq, eps):
+    dev = q.device
+    for name, t in (("q", q), ("k", k)):
+        _chk(t, q.dtype, f"{what}: {name}")
+        if t.dim() != 4 or t.device != dev:
+            raise N.NativeError(f"{what}: {name} must be [batch, length, heads, head dim] on {dev}, got {tuple(t.shape)} on {t.device}")
+    if q.dtype not in _TYPE:
+        raise N.NativeError(f"{what}: bf16, fp16 or f32, got {q.dtype}")
+    B, L, H, D = q.shape
+    if k.shape[:2] != (B, L) or k.shape[3] != D or H < 1 or k.shape[2] < 1:
+        raise N.NativeError(f"{what}: shapes q {tuple(q.shape)}, k {tuple(k.shape)}")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _chk(t, F32, f"{what}: {name}")
+        if t.shape != (D,) or t.device != dev:
+            raise N.NativeError(f"{what}: {name} must be [{D}] on {dev}, got {tuple(t.shape)} on {t.device}")
+    _chk(inv_freq, F32, f"{what}: inv_freq")
+    R = 2 * inv_freq.numel()
+    if inv_freq.dim() != 1 or inv_freq.device != dev or D < 8 or D > 256 or D % 8 or not 2 <= R <= D:
+        raise N.NativeError(f"{what}: head dim {D} (a multiple of 8 up to 256) with inv_freq {tuple(inv_freq.shape)} (1 .. head dim / 2)")
+    _chk(positions, None, f"{what}: positions")
+    if positions.dtype not in _INT_BYTES or positions.device != dev or positions.shape not in ((B, L), (L,)):
+        raise N.NativeError(f"{what}: positions must be int32 or int64 [{B}, {L}] or [{L}] on {dev}, got {positions.dtype} "
+                            f"{tuple(positions.shape)} on {positions.device}")
+    if L > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise N.NativeError(f"{what}: eps must be finite and not negative, got {eps}")
+    return _last1(q), _last1(k), q_weight.contiguous(), k_weight.contiguous(), positions, inv_freq.contiguous()
+
+
+def _last1(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _rope_desc(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, eps, interleaved, gq=None, gk=None, dqw=None, dkw=None):
+    B, L, H, D = q.shape
+    z = (0, 0, 0)
+    pos_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
+    return N.RopeDesc(ptr(q), ptr(k), ptr(q_weight), ptr(k_weight), ptr(positions), ptr(inv_freq), ptr(q_out), ptr(k_out), ptr(gq),
+                      ptr(gk), ptr(dqw), ptr(dkw), None, 0, *_strides(q), *_strides(k), *_strides(q_out), *_strides(k_out),
+                      *(z if gq is None else _strides(gq)), *(z if gk is None else _strides(gk)), pos_stride, B, L, H, k.shape[2], D,
+                      2 * inv_freq.numel(), _TYPE[q.dtype], bool(interleaved), _INT_BYTES[positions.dtype], eps)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """(q_out, k_out): each head of q [B, L, H, D] and k [B, L, Hk, D] (bf16, fp16 or f32; any batch / row / head strides; D a
+    multiple of 8 up to 256) divided by its root mean square (eps inside the root), times its weight (f32 [D]), then its first
+    R = 2 len(inv_freq) dims rotated by positions * inv_freq: pairs (i, R/2 + i), or (2i, 2i + 1) with interleaved.
+    positions int32 / int64 [B, L] or [L]; inv_freq f32; the angles are formed in 64 bits, all else in f32 with one rounding."""
+    q, k, q_weight, k_weight, positions, inv_freq = _rope_args("qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, eps)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    d = _rope_desc(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, eps, interleaved)
+    _call_on("lrce_qk_norm_rope_fwd", q, ctypes.byref(d), stream_of(q))
+    return q_out, k_out
+
+
+def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rope() for the gradients of its outputs; the other arguments as there.  The
+    weights' gradients (f32) are summed in a fixed order."""
+    what = "qk_norm_rope_bwd"
+    q, k, q_weight, k_weight, positions, inv_freq = _rope_args(what, q, k, q_weight, k_weight, positions, inv_freq, eps)
+    for name, g, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
+        _chk(g, q.dtype, f"{what}: {name}")
+        if g.shape != x.shape or g.device != q.device:
+            raise N.NativeError(f"{what}: {name} must be {tuple(x.shape)} on {q.device}, got {tuple(g.shape)} on {g.device}")
+    dq_out, dk_out = _last1(dq_out), _last1(dk_out)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dqw = torch.empty_like(q_weight)
+    dkw = torch.empty_like(k_weight)
+    d = _rope_desc(q, k, q_weight, k_weight, positions, inv_freq, dq, dk, eps, interleaved, dq_out, dk_out, dqw, dkw)
+    n = N.lib().lrce_qk_norm_rope_bwd_workspace(ctypes.byref(d))
+    ws = torch.empty(max(n, 0), dtype=F32, device=q.device)
+    d.workspace, d.workspace_elems = ptr(ws), n
+    _call_on("lrce_qk_norm_rope_bwd", q, ctypes.byref(d), stream_of(q))
+    return dq, dk, dqw, dkw
+
+
+# ---- embedding lookup and its gradient by sorted tokens (csrc/embedding.hip) -------------------------
+def _embed_ids(what, ids, dev):
+    _chk(ids, None, f"{what}: ids")
+    if ids.dtype not in _INT_BYTES or ids.device != dev:
+        raise N.NativeError(f"{what}: ids must be int32 or int64 on {dev}, got {ids.dtype} on {ids.device}")
+    return ids.contiguous()
+
+
+def embedding(ids, weight, scale=1.0, out_dtype=None):
+    """scale * weight[ids]: ids (any shape) int32 / int64, weight [rows, cols] bf16, fp16 or f32 (rows may be strided); the result
+    has weight's type, or out_dtype where weight is f32.  An id outside the table gives a row of NaN (no host check)."""
+    _chk(weight, None, "embedding: weight")
+    out_dtype = weight.dtype if out_dtype is None else out_dtype
+    if weight.dim() != 2 or weight.dtype not in _TYPE or out_dtype not in _TYPE or (weight.dtype != F32 and out_dtype != weight.dtype):
+        raise N.NativeError(f"embedding: weight [rows, cols] of bf16, fp16 or f32, got {tuple(weight.shape)} {weight.dtype} -> {out_dtype}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise N.NativeError(f"embedding: an empty table {tuple(weight.shape)}")
+    ids = _embed_ids("embedding", ids, weight.device)
+    if weight.shape[1] > 1 and weight.stride(1) != 1 or weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]:
+        weight = weight.contiguous()
+    rows, cols = weight.shape
+    y = torch.empty((*ids.shape, cols), dtype=out_dtype, device=weight.device)
+    _call_on("lrce_embedding_fwd", y, ptr(ids), _INT_BYTES[ids.dtype], ids.numel(), ptr(weight), weight.stride(0) if rows > 1 else cols, rows,
+             cols, _TYPE[weight.dtype], ptr(y), _TYPE[out_dtype], float(scale), stream_of(y))
+    return y
+
+
+def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=-1, dw=None):
+    """The gradient of embedding()'s table for dy [*ids.shape, cols] (bf16, fp16 or f32): f32 [rows, cols], row v = scale * the sum
+    of dy over the places where ids is v, in their order (the same bits each time); padding_idx (-1: none) and ids outside the
+    table have none.  dw: a contiguous f32 [rows, cols] the gradient is added to (and returned) instead of a new tensor."""
+    _chk(dy, None, "embedding_bwd: dy")
+    if dy.dtype not in _TYPE:
+        raise N.NativeError(f"embedding_bwd: dy must be bf16, fp16 or f32, got {dy.dtype}")
+    ids = _embed_ids("embedding_bwd", ids, dy.device)
+    if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] < 1 or rows < 1:
+        raise N.NativeError(f"embedding_bwd: dy {tuple(dy.shape)} for ids {tuple(ids.shape)} and {rows} rows")
+    cols, n = dy.shape[-1], ids.numel()
+    dy = dy.contiguous()
+    add = dw is not None
+    if add:
+        _chk(dw, F32, "embedding_bwd: dw")
+        if dw.shape != (rows, cols) or not dw.is_contiguous() or dw.device != dy.device or dw.data_ptr() % 16:
+            raise N.NativeError(f"embedding_bwd: dw must be a contiguous f32 {(rows, cols)} on {dy.device}")
+    else:
+        dw = torch.empty((rows, cols), dtype=F32, device=dy.device)
+    k = N.lib().lrce_embedding_bwd_workspace(n, rows, cols)
+    ws = torch.empty(max(k, 0), dtype=F32, device=dy.device)
+    _call_on("lrce_embedding_bwd", dw, ptr(ids), _INT_BYTES[ids.dtype], n, ptr(dy), _TYPE[dy.dtype], ptr(dw), rows, cols, float(scale),
+             int(padding_idx), int(add), ptr(ws), k, stream_of(dw))
+    return dw
+
+
 # ---- recurrent decoder: per-head fused attention blocks (csrc/decoder.hip) -------------------------
 DEC_MAX_ROWS = 64
 _DEC_WS = {}
