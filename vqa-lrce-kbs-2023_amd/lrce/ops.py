@@ -29,12 +29,23 @@ Ops (reference modules they replace):
   decoder_recurrent(video, text, params) -> s     FusionTransformer.forward   fusionv3.py:27-51
                                                   (the recurrent 12-layer decoder over S steps, eval
                                                   mode; text None: FusionVideo, fusionv3.py:70-88)
+  attention(q, k, v, key_mask?, causal, scale?) -> (out, lse)
+                                                  multi-head attention at general lengths (head dims 32 - 128,
+                                                  shared key heads, key mask, causality, single tokens)
+  attention_backward(dout, q, k, v, out, lse, key_mask?, causal, scale?) -> (dq, dk, dv)
+  qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved) -> (q_out, k_out)
+                                                  per-head RMS norm + rotary position embedding in one pass
+  qk_norm_rope_backward(dq_out, dk_out, q, k, ...) -> (dq, dk, dq_weight, dk_weight)
+  embedding(ids, weight, scale, padding_idx) -> y lookup with scaling (nn.Embedding)
+  embedding_backward(dy, ids, rows, scale, padding_idx) -> dweight
+                                                  its gradient by sorted tokens: the same bits each time
 
 Autograd (torch.library.register_autograd): linear, layer_norm, window_attention and patch_embed are
 differentiable through the same native kernels (linear: dX / dW GEMMs + fused bias gradient;
 layer_norm: lrce_layernorm_bwd w.r.t. y; window_attention: window_attention_backward w.r.t. out —
 its qkv / lse outputs are saved activations, marked non-differentiable; patch_embed: w.r.t. the conv
-and LayerNorm parameters, the clips are data).  decoder_recurrent is a forward (inference) op; the
+and LayerNorm parameters, the clips are data; attention: attention_backward w.r.t. out, lse is a saved
+activation, marked non-differentiable; qk_norm_rope and embedding: their backward ops).  decoder_recurrent is a forward (inference) op; the
 model's training path differentiates the decoder as one autograd node (lrce/models/fusionv3.py).
 """
 from typing import List, Optional, Tuple
@@ -286,6 +297,127 @@ def _pe_backward(ctx, dx, dpatches, dy_, dmean, drstd):
 patch_embed.register_autograd(_pe_backward, setup_context=_pe_setup)
 
 
+@torch.library.custom_op("lrce::attention", mutates_args=())
+def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None, causal: bool = False,
+              scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
+    """softmax(scale q k^T) v per head over the keys a row may see (lrce_attn_fwd): q [B, Lq, H, D], k / v [B, Lk, Hk, D] bf16 or
+    fp16, key_mask [B, Lk] (0 = hidden), causal: j <= i + Lk - Lq.  Returns (out [B, Lq, H, D], lse f32 [B, H, Lq]); see
+    kernels.attention."""
+    return K.attention(q, k, v, key_mask, causal, scale)
+
+
+@attention.register_fake
+def _(q, k, v, key_mask=None, causal=False, scale=None):
+    B, Lq, H, D = q.shape
+    return q.new_empty((B, Lq, H, D)), q.new_empty((B, H, Lq), dtype=torch.float32)
+
+
+@torch.library.custom_op("lrce::attention_backward", mutates_args=())
+def attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, key_mask: Optional[Tensor] = None,
+                       causal: bool = False, scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dq, dk, dv) of attention given d(out); the weights are recomputed from lse (lrce_attn_bwd)."""
+    return K.attention_bwd(dout, q, k, v, out, lse, key_mask, causal, scale)
+
+
+@attention_backward.register_fake
+def _(dout, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+def _attn_setup(ctx, inputs, output):
+    q, k, v, key_mask, causal, scale = inputs
+    out, lse = output
+    ctx.save_for_backward(q, k, v, out, lse, key_mask)
+    ctx.causal, ctx.scale = causal, scale
+    ctx.mark_non_differentiable(lse)
+
+
+def _attn_backward(ctx, dout, dlse):
+    q, k, v, out, lse, key_mask = ctx.saved_tensors
+    dq, dk, dv = attention_backward(dout, q, k, v, out, lse, key_mask, ctx.causal, ctx.scale)
+    return dq, dk, dv, None, None, None
+
+
+attention.register_autograd(_attn_backward, setup_context=_attn_setup)
+
+
+@torch.library.custom_op("lrce::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, positions: Tensor, inv_freq: Tensor, eps: float = 1e-6,
+                 interleaved: bool = False) -> Tuple[Tensor, Tensor]:
+    """Per-head RMS norm of q [B, L, H, D] and k [B, L, Hk, D] times f32 weights [D], then the rotary position embedding of the first
+    2 len(inv_freq) dims (lrce_qk_norm_rope_fwd); see kernels.qk_norm_rope."""
+    return K.qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("lrce::qk_norm_rope_backward", mutates_args=())
+def qk_norm_rope_backward(dq_out: Tensor, dk_out: Tensor, q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, positions: Tensor,
+                          inv_freq: Tensor, eps: float = 1e-6,
+                          interleaved: bool = False) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rope (lrce_qk_norm_rope_bwd; the weights' gradients f32)."""
+    return K.qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+
+
+@qk_norm_rope_backward.register_fake
+def _(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape), q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
+
+
+def _rope_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:6])
+    ctx.eps, ctx.interleaved = inputs[6], inputs[7]
+
+
+def _rope_backward(ctx, dq_out, dk_out):
+    q, k = ctx.saved_tensors[:2]
+    dq_out = torch.zeros_like(q) if dq_out is None else dq_out
+    dk_out = torch.zeros_like(k) if dk_out is None else dk_out
+    return (*qk_norm_rope_backward(dq_out, dk_out, *ctx.saved_tensors, ctx.eps, ctx.interleaved), None, None, None, None)
+
+
+qk_norm_rope.register_autograd(_rope_backward, setup_context=_rope_setup)
+
+
+@torch.library.custom_op("lrce::embedding", mutates_args=())
+def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int = -1) -> Tensor:
+    """scale * weight[ids] (lrce_embedding_fwd); padding_idx: the row without a gradient (-1: none), as nn.Embedding's."""
+    return K.embedding(ids, weight, scale)
+
+
+@embedding.register_fake
+def _(ids, weight, scale=1.0, padding_idx=-1):
+    return weight.new_empty((*ids.shape, weight.shape[1]))
+
+
+@torch.library.custom_op("lrce::embedding_backward", mutates_args=())
+def embedding_backward(dy: Tensor, ids: Tensor, rows: int, scale: float = 1.0, padding_idx: int = -1) -> Tensor:
+    """The table's gradient, f32 [rows, cols], by sorted tokens (lrce_embedding_bwd)."""
+    return K.embedding_bwd(dy, ids, rows, scale, padding_idx)
+
+
+@embedding_backward.register_fake
+def _(dy, ids, rows, scale=1.0, padding_idx=-1):
+    return dy.new_empty((rows, dy.shape[-1]), dtype=torch.float32)
+
+
+def _embed_setup(ctx, inputs, output):
+    ids, weight, scale, padding_idx = inputs
+    ctx.save_for_backward(ids)
+    ctx.rows, ctx.dtype, ctx.scale, ctx.padding_idx = weight.shape[0], weight.dtype, scale, padding_idx
+
+
+def _embed_backward(ctx, dy):
+    dw = embedding_backward(dy, *ctx.saved_tensors, ctx.rows, ctx.scale, ctx.padding_idx)
+    return None, dw.to(ctx.dtype), None, None
+
+
+embedding.register_autograd(_embed_backward, setup_context=_embed_setup)
+
+
 _DEC = {}
 
 
@@ -338,4 +470,5 @@ def _(video, text, params):
 def registered() -> List[str]:
     """The lrce operators the dispatcher knows."""
     return ["linear", "linear_dx", "linear_dw_", "layer_norm", "window_attention", "window_attention_backward",
-            "patch_embed", "decoder_recurrent"]
+            "patch_embed", "decoder_recurrent", "attention", "attention_backward", "qk_norm_rope", "qk_norm_rope_backward",
+            "embedding", "embedding_backward"]
