@@ -423,7 +423,7 @@ typedef struct LrceRopeDesc {
 } LrceRopeDesc;
 
 int lrce_qk_norm_rope_fwd(const LrceRopeDesc* desc, void* stream);
-int64_t lrce_qk_norm_rope_bwd_workspace(const LrceRopeDesc* desc);
+int64_t lrce_qk_norm_rope_bwd_workspace(int64_t tokens, int D);  /* tokens = B * L; negative: bad sizes */
 int lrce_qk_norm_rope_bwd(const LrceRopeDesc* desc, void* stream);
 
 /* Embedding lookup y[i][:] = scale * w[ids[i]][:] (types 0 bf16, 1 fp16, 2 f32; y has w's type, or any where w is f32; ids int32 /

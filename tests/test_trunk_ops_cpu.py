@@ -75,7 +75,13 @@ def test_rope_refusals(over, word):
     assert word in L.lrce_last_error(), L.lrce_last_error()
     d = rope(gq=A, gk=A, dq_weight=A, dk_weight=A, **over)
     assert L.lrce_qk_norm_rope_bwd(ctypes.byref(d), None) == 1 and word in L.lrce_last_error()
-    assert L.lrce_qk_norm_rope_bwd_workspace(ctypes.byref(d)) == -1
+
+
+def test_rope_workspace():
+    _, L = lib()
+    for tokens, D in ((-1, 64), (4, 12), (4, 264), (4, 0)):
+        assert L.lrce_qk_norm_rope_bwd_workspace(tokens, D) == -1
+    assert L.lrce_qk_norm_rope_bwd_workspace(0, 64) == 128
 
 
 def test_rope_backward_needs_gradients_and_a_workspace():

@@ -292,11 +292,8 @@ int rope_check(const LrceRopeDesc* d, bool bwd, const char* what) {
   return LRCE_OK;
 }
 
-int rope_wgs(const LrceRopeDesc* d, int tpw) {
-  // the backward leaves a row of partial sums a workgroup: 4 workgroups a CU
-  const int64_t need = ((int64_t)d->B * d->L + 4 * tpw - 1) / (4 * tpw);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(need, 1024));
-}
+// The backward leaves a row of partial sums a workgroup, four waves of at least a token each: up to 4 workgroups a CU
+int64_t rope_wgs(int64_t tokens) { return std::max<int64_t>(1, std::min<int64_t>((tokens + 3) / 4, 1024)); }
 
 struct RopePlan { int vec, lgrp, gpt, tpw; };
 
@@ -375,9 +372,9 @@ extern "C" int lrce_qk_norm_rope_fwd(const LrceRopeDesc* d, void* stream) {
   return lrce_check_launch("qk_norm_rope");
 }
 
-extern "C" int64_t lrce_qk_norm_rope_bwd_workspace(const LrceRopeDesc* d) {
-  if (rope_check(d, true, "qk_norm_rope_bwd_workspace")) return -1;
-  return (int64_t)rope_wgs(d, rope_plan(d, true).tpw) * 2 * d->D;
+extern "C" int64_t lrce_qk_norm_rope_bwd_workspace(int64_t tokens, int D) {
+  if (tokens < 0 || D < 8 || D > 256 || D % 8) return -1;
+  return rope_wgs(tokens) * 2 * D;
 }
 
 extern "C" int lrce_qk_norm_rope_bwd(const LrceRopeDesc* d, void* stream) {
@@ -385,7 +382,7 @@ extern "C" int lrce_qk_norm_rope_bwd(const LrceRopeDesc* d, void* stream) {
   const RopePlan f = rope_plan(d, true);
   RopeP p;
   rope_fill(d, f, p);
-  p.nwg = rope_wgs(d, f.tpw);
+  p.nwg = (int)rope_wgs(p.tokens);
   if (!d->workspace || d->workspace_elems < (int64_t)p.nwg * 2 * d->D)
     return lrce_fail(LRCE_E_ARG, "qk_norm_rope_bwd: a workspace of %lld floats is needed", (long long)p.nwg * 2 * d->D);
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -229,13 +229,13 @@ _SIGS = {
     "lrce_layernorm_bwd_f16s_deferred": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _F, _U64, _P, _I64, _P, _P],
     "lrce_mha_fwd": [ctypes.POINTER(MhaDesc), _P],
     "lrce_mha_bwd": [ctypes.POINTER(MhaDesc), _P],
-    "lrce_attn_fwd": [ctypes.POINTER(AttnDesc), _P],
-    "lrce_attn_bwd": [ctypes.POINTER(AttnDesc), _P],
+    "lrce_attn_fwd": [_P, _P],
+    "lrce_attn_bwd": [_P, _P],
     "lrce_attn_fwd_workspace": [ctypes.POINTER(AttnDesc)],
     "lrce_attn_bwd_workspace": [ctypes.POINTER(AttnDesc)],
-    "lrce_qk_norm_rope_fwd": [ctypes.POINTER(RopeDesc), _P],
-    "lrce_qk_norm_rope_bwd": [ctypes.POINTER(RopeDesc), _P],
-    "lrce_qk_norm_rope_bwd_workspace": [ctypes.POINTER(RopeDesc)],
+    "lrce_qk_norm_rope_fwd": [_P, _P],
+    "lrce_qk_norm_rope_bwd": [_P, _P],
+    "lrce_qk_norm_rope_bwd_workspace": [_I64, _I],
     "lrce_embedding_fwd": [_P, _I, _I64, _P, _I64, _I64, _I, _I, _P, _I, _F, _P],
     "lrce_embedding_bwd_workspace": [_I64, _I64, _I],
     "lrce_embedding_bwd": [_P, _I, _I64, _P, _I, _P, _I64, _I, _F, _I64, _I, _P, _I64, _P],

@@ -5,7 +5,9 @@ Conventions: activations are 2-D row-major [rows, features]; weights are nn.Line
 [out, in]; "bf16" tensors are torch.bfloat16; gradients of parameters are f32 and accumulated.
 """
 import ctypes
+import functools
 import math
+import struct
 
 import torch
 
@@ -654,32 +656,48 @@ def mha_desc(q, Lq, *, k1, v1, lk1, ld_kv1, stride_kv1_b, kv1_bdiv=1, k2=None, v
 
 
 # ---- attention at general lengths (csrc/attention.hip, attention_bwd.hip) ---------------------------
+# The operators below are called on single tokens too, where the host's share of a call is most of its time: one test of
+# the arguments (the refusal is worded only when it fails), descriptors packed in one go (the layout of the C structs,
+# N.AttnDesc / N.RopeDesc), workspace sizes remembered by the sizes that they follow from.
 _MASK_BYTES = {torch.bool: 1, torch.uint8: 1, torch.int8: 1, torch.int32: 4, torch.int64: 8}
+_INT_BYTES = {torch.int32: 4, torch.int64: 8}
+_TYPE = {BF16: 0, F16: 1, F32: 2}
+_ATTN_PACK = struct.Struct("6P13q9ifPq4P12q").pack
+_ROPE_PACK = struct.Struct("13Pq18qq9if").pack
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _call_on(name, t, *args):
-    """N.call with t's device as the current one: a launch goes to the device of its stream."""
-    if t.device.index == torch.cuda.current_device():
-        return call(name, *args)
-    with torch.cuda.device(t.device):
-        return call(name, *args)
+    """N.call on t's current stream, with t's device as the current one: a launch goes to the device of its stream."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        return call(name, *args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return call(name, *args, _raw_stream(dev))
 
 
-def _strides(t):
-    """Strides of all but the last axis; 0 for an axis of length 1, whose stride says nothing."""
-    return [st if n > 1 else 0 for st, n in zip(t.stride()[:-1], t.shape[:-1])]
+def _head_rows(t):
+    """(t, strides of batch, row, head) of [B, L, H, D] with a contiguous last axis; the stride of an axis of length 1 says
+    nothing and counts as 0."""
+    if t.is_contiguous():
+        _, n, h, d = t.shape
+        return t, n * h * d, h * d, d
+    sb, sl, sh, sd = t.stride()
+    b, n, h, d = t.shape
+    if sd != 1 and d > 1:
+        return _head_rows(t.contiguous())
+    return t, sb if b > 1 else 0, sl if n > 1 else 0, sh if h > 1 else 0
 
 
-def _rows16(t):
-    """t, or a contiguous copy where its rows are not whole 16-byte pieces as the kernels read them."""
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and not any(
-            s % 8 or s >= 1 << 23 for s in _strides(t)[1:]) and _strides(t)[0] % 8 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _head_rows16(t):
+    """_head_rows of t, or of a copy where its rows are not the whole 16-byte pieces that the kernels read."""
+    r = _head_rows(t)
+    if (r[1] | r[2] | r[3]) & 7 or r[2] >= 1 << 23 or r[0].data_ptr() & 15:
+        return _head_rows(t.clone(memory_format=torch.contiguous_format))
+    return r
 
 
-def _attn_args(what, q, k, v, key_mask, causal, scale):
-    """Checked (q, k, v, mask, scale) of the attention operators."""
+def _attn_refuse(what, q, k, v, key_mask, scale):
     for name, t in (("q", q), ("k", k), ("v", v)):
         _chk(t, q.dtype, f"{what}: {name}")
         if t.device != q.device:
@@ -688,33 +706,39 @@ def _attn_args(what, q, k, v, key_mask, causal, scale):
             raise N.NativeError(f"{what}: {name} must be [batch, length, heads, head dim], got {tuple(t.shape)}")
     if q.dtype not in (BF16, F16):
         raise N.NativeError(f"{what}: bf16 or fp16, got {q.dtype}")
-    B, Lq, H, D = q.shape
-    Lk, Hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hk < 1 or H < 1 or H % Hk:
-        raise N.NativeError(f"{what}: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if D not in (32, 64, 96, 128):
-        raise N.NativeError(f"{what}: head dim {D} (32, 64, 96 or 128)")
-    if key_mask is not None:
-        if not key_mask.is_cuda or key_mask.device != q.device or key_mask.dtype not in _MASK_BYTES:
-            raise N.NativeError(f"{what}: key_mask must be bool or integer on {q.device}")
-        if key_mask.shape != (B, Lk):
-            raise N.NativeError(f"{what}: key_mask must be {(B, Lk)}, got {tuple(key_mask.shape)}")
-        if Lk > 1 and key_mask.stride(1) != 1:
-            key_mask = key_mask.contiguous()
-    scale = float(D) ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise N.NativeError(f"{what}: scale must be positive and finite, got {scale}")
-    return _rows16(q), _rows16(k), _rows16(v), key_mask, scale
+    if key_mask is not None and (key_mask.device != q.device or key_mask.dtype not in _MASK_BYTES):
+        raise N.NativeError(f"{what}: key_mask must be bool or integer on {q.device}, got {key_mask.dtype} on {key_mask.device}")
+    if key_mask is not None and key_mask.shape != (q.shape[0], k.shape[1]):
+        raise N.NativeError(f"{what}: key_mask must be {(q.shape[0], k.shape[1])}, got {tuple(key_mask.shape)}")
+    raise N.NativeError(f"{what}: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} (head dim 32, 64, 96 or 128; query "
+                        f"heads a multiple of the key heads), scale {scale} (positive and finite)")
 
 
-def _attn_desc(q, k, v, out, lse, key_mask, causal, scale, dout=None, dq=None, dk=None, dv=None):
+def _attn_args(what, q, k, v, key_mask, scale):
+    """Checked sizes (B, Lq, H, D, Lk, Hk), mask, scale of the attention operators."""
+    dt, dev, ks = q.dtype, q.get_device(), k.shape
+    if not (q.is_cuda and (dt is BF16 or dt is F16) and k.dtype is dt and v.dtype is dt and k.get_device() == dev == v.get_device()
+            and q.dim() == 4 == len(ks) and ks == v.shape):
+        _attn_refuse(what, q, k, v, key_mask, scale)
     B, Lq, H, D = q.shape
-    m = key_mask
-    grads = (dout, dq, dk, dv)
-    return N.AttnDesc(ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(m), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
-                      0 if m is None or B <= 1 else m.stride(0), B, H, k.shape[2], Lq, k.shape[1], D, q.dtype == F16, bool(causal),
-                      0 if m is None else _MASK_BYTES[m.dtype], scale, None, 0, *(ptr(t) for t in grads),
-                      *(s for t in grads for s in (_strides(t) if t is not None else (0, 0, 0))))
+    Bk, Lk, Hk, Dk = ks
+    scale = D ** -0.5 if scale is None and D > 0 else float(scale or 0.0)
+    if not (Bk == B and Dk == D and D in (32, 64, 96, 128) and Hk > 0 and H > 0 and H % Hk == 0 and 0.0 < scale < math.inf
+            and (key_mask is None or (key_mask.get_device() == dev and key_mask.dtype in _MASK_BYTES and key_mask.shape == (B, Lk)))):
+        _attn_refuse(what, q, k, v, key_mask, scale)
+    if key_mask is not None and Lk > 1 and key_mask.stride(1) != 1:
+        key_mask = key_mask.contiguous()
+    return B, Lq, H, D, Lk, Hk, key_mask, scale
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_ws(bwd, B, H, Hk, Lq, Lk, D):
+    """Floats of workspace (a function of the sizes; the descriptor's pointers are not looked at)."""
+    d = N.AttnDesc(q=16, k=16, v=16, out=16, lse=16, B=B, H=H, Hk=Hk, Lq=Lq, Lk=Lk, D=D, scale=1.0)
+    n = getattr(N.lib(), "lrce_attn_bwd_workspace" if bwd else "lrce_attn_fwd_workspace")(ctypes.byref(d))
+    if n < 0:
+        raise N.NativeError(N.lib().lrce_last_error().decode())
+    return n
 
 
 def attention(q, k, v, key_mask=None, causal=False, scale=None):
@@ -723,91 +747,79 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
     key_mask [B, Lk] (bool or integer, 0 = hidden); causal: row i sees the keys j <= i + Lk - Lq; scale (positive): D ** -0.5 by
     default.  A row that sees no key gives 0 and lse -inf.  k and v may hold anything at keys that key_mask hides; at keys
     that only causality hides they must be finite.  lse is the natural logarithm of the row's sum, for attention_bwd."""
-    q, k, v, key_mask, scale = _attn_args("attention", q, k, v, key_mask, causal, scale)
-    B, Lq, H, D = q.shape
-    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Lq), dtype=F32, device=q.device)
-    d = _attn_desc(q, k, v, out, lse, key_mask, causal, scale)
-    n = N.lib().lrce_attn_fwd_workspace(ctypes.byref(d))
-    if n > 0:
-        ws = torch.empty(n, dtype=F32, device=q.device)
-        d.workspace, d.workspace_elems = ptr(ws), n
-    _call_on("lrce_attn_fwd", q, ctypes.byref(d), stream_of(q))
+    B, Lq, H, D, Lk, Hk, m, scale = _attn_args("attention", q, k, v, key_mask, scale)
+    q, *qs = _head_rows16(q)
+    k, *ks = _head_rows16(k)
+    v, *vs = _head_rows16(v)
+    out = q.new_empty((B, Lq, H, D))
+    lse = q.new_empty((B, H, Lq), dtype=F32)
+    n = _attn_ws(False, B, H, Hk, Lq, Lk, D)
+    ws = q.new_empty(n, dtype=F32) if n else None
+    _call_on("lrce_attn_fwd", q, _ATTN_PACK(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0 if m is None else m.data_ptr(), *qs, *ks, *vs,
+        Lq * H * D, H * D, D, 0 if m is None or B < 2 else m.stride(0), B, H, Hk, Lq, Lk, D, q.dtype is F16, bool(causal),
+        0 if m is None else _MASK_BYTES[m.dtype], scale, ws.data_ptr() if n else 0, n, *(0,) * 16))
     return out, lse
 
 
 def attention_bwd(dout, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
     """(dq, dk, dv) of attention() for dout, with the forward's out and lse; the arguments as there.  Sums over the query
     heads that share a key head are formed in f32; the result does not depend on timing."""
-    q, k, v, key_mask, scale = _attn_args("attention_bwd", q, k, v, key_mask, causal, scale)
-    B, Lq, H, D = q.shape
-    for name, t in (("dout", dout), ("out", out)):
-        _chk(t, q.dtype, f"attention_bwd: {name}")
-        if t.shape != q.shape or t.device != q.device:
-            raise N.NativeError(f"attention_bwd: {name} must be {tuple(q.shape)} on {q.device}, got {tuple(t.shape)} on {t.device}")
-    _chk(lse, F32, "attention_bwd: lse")
-    if lse.shape != (B, H, Lq) or lse.device != q.device:
-        raise N.NativeError(f"attention_bwd: lse must be {(B, H, Lq)} on {q.device}, got {tuple(lse.shape)} on {lse.device}")
-    dout, out, lse = _rows16(dout), _rows16(out), lse.contiguous()
-    dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    d = _attn_desc(q, k, v, out, lse, key_mask, causal, scale, dout, dq, dk, dv)
-    n = N.lib().lrce_attn_bwd_workspace(ctypes.byref(d))
-    if n > 0:
-        ws = torch.empty(n, dtype=F32, device=q.device)
-        d.workspace, d.workspace_elems = ptr(ws), n
-    _call_on("lrce_attn_bwd", q, ctypes.byref(d), stream_of(q))
+    B, Lq, H, D, Lk, Hk, m, scale = _attn_args("attention_bwd", q, k, v, key_mask, scale)
+    dev, shape = q.get_device(), q.shape
+    if not (dout.dtype is q.dtype and out.dtype is q.dtype and dout.shape == shape and out.shape == shape and dout.get_device() == dev
+            and out.get_device() == dev and lse.dtype is F32 and lse.shape == (B, H, Lq) and lse.get_device() == dev):
+        raise N.NativeError("attention_bwd: " + ", ".join(
+            f"{n} {tuple(t.shape)} {t.dtype} on {t.device}" for n, t in (("dout", dout), ("out", out), ("lse", lse)))
+            + f" for q {tuple(shape)} {q.dtype} on {q.device} (lse: f32 [batch, heads, length])")
+    q, *qs = _head_rows16(q)
+    k, *ks = _head_rows16(k)
+    v, *vs = _head_rows16(v)
+    out, *os_ = _head_rows16(out)
+    dout, *gs = _head_rows16(dout)
+    lse = lse.contiguous()
+    dq = q.new_empty((B, Lq, H, D))
+    dk = q.new_empty((B, Lk, Hk, D))
+    dv = q.new_empty((B, Lk, Hk, D))
+    n = _attn_ws(True, B, H, Hk, Lq, Lk, D)
+    ws = q.new_empty(n, dtype=F32)
+    kv = (Lk * Hk * D, Hk * D, D)
+    _call_on("lrce_attn_bwd", q, _ATTN_PACK(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0 if m is None else m.data_ptr(), *qs, *ks, *vs, *os_,
+        0 if m is None or B < 2 else m.stride(0), B, H, Hk, Lq, Lk, D, q.dtype is F16, bool(causal),
+        0 if m is None else _MASK_BYTES[m.dtype], scale, ws.data_ptr(), n, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        *gs, Lq * H * D, H * D, D, *kv, *kv))
     return dq, dk, dv
 
 
 # ---- query / key norm with the position rotation (csrc/qk_rope.hip) ---------------------------------
-_TYPE = {BF16: 0, F16: 1, F32: 2}
-_INT_BYTES = {torch.int32: 4, torch.int64: 8}
-
-
-def _rope_args(what, q, k, q_weight, k_weight, positions, inv_freq, eps):
+def _rope_refuse(what, q, k, q_weight, k_weight, positions, inv_freq, eps):
     dev = q.device
     for name, t in (("q", q), ("k", k)):
         _chk(t, q.dtype, f"{what}: {name}")
         if t.dim() != 4 or t.device != dev:
             raise N.NativeError(f"{what}: {name} must be [batch, length, heads, head dim] on {dev}, got {tuple(t.shape)} on {t.device}")
-    if q.dtype not in _TYPE:
-        raise N.NativeError(f"{what}: bf16, fp16 or f32, got {q.dtype}")
-    B, L, H, D = q.shape
-    if k.shape[:2] != (B, L) or k.shape[3] != D or H < 1 or k.shape[2] < 1:
-        raise N.NativeError(f"{what}: shapes q {tuple(q.shape)}, k {tuple(k.shape)}")
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("inv_freq", inv_freq)):
         _chk(t, F32, f"{what}: {name}")
-        if t.shape != (D,) or t.device != dev:
-            raise N.NativeError(f"{what}: {name} must be [{D}] on {dev}, got {tuple(t.shape)} on {t.device}")
-    _chk(inv_freq, F32, f"{what}: inv_freq")
-    R = 2 * inv_freq.numel()
-    if inv_freq.dim() != 1 or inv_freq.device != dev or D < 8 or D > 256 or D % 8 or not 2 <= R <= D:
-        raise N.NativeError(f"{what}: head dim {D} (a multiple of 8 up to 256) with inv_freq {tuple(inv_freq.shape)} (1 .. head dim / 2)")
-    _chk(positions, None, f"{what}: positions")
-    if positions.dtype not in _INT_BYTES or positions.device != dev or positions.shape not in ((B, L), (L,)):
-        raise N.NativeError(f"{what}: positions must be int32 or int64 [{B}, {L}] or [{L}] on {dev}, got {positions.dtype} "
-                            f"{tuple(positions.shape)} on {positions.device}")
-    if L > 1 and positions.stride(-1) != 1:
-        positions = positions.contiguous()
-    if not (eps >= 0.0 and math.isfinite(eps)):
-        raise N.NativeError(f"{what}: eps must be finite and not negative, got {eps}")
-    return _last1(q), _last1(k), q_weight.contiguous(), k_weight.contiguous(), positions, inv_freq.contiguous()
+    raise N.NativeError(
+        f"{what}: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} (bf16, fp16 or f32, head dim a multiple of 8 up to 256), weights "
+        f"{tuple(q_weight.shape)}, {tuple(k_weight.shape)}, positions {positions.dtype} {tuple(positions.shape)} (int32 or int64, [batch, "
+        f"length] or [length]), inv_freq {tuple(inv_freq.shape)} (1 to head dim / 2), eps {eps}, all on one device")
 
 
-def _last1(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _rope_desc(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, eps, interleaved, gq=None, gk=None, dqw=None, dkw=None):
+def _rope_args(what, q, k, q_weight, k_weight, positions, inv_freq, eps):
+    """(B, L, H, Hk, D) after the checks."""
+    dev, dt, ks = q.get_device(), q.dtype, k.shape
+    if not (q.is_cuda and dt in _TYPE and k.dtype is dt and q.dim() == 4 == len(ks)
+            and k.get_device() == q_weight.get_device() == k_weight.get_device() == positions.get_device() == inv_freq.get_device() == dev
+            and q_weight.dtype is k_weight.dtype is inv_freq.dtype is F32 and positions.dtype in _INT_BYTES and inv_freq.dim() == 1):
+        _rope_refuse(what, q, k, q_weight, k_weight, positions, inv_freq, eps)
     B, L, H, D = q.shape
-    z = (0, 0, 0)
-    pos_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
-    return N.RopeDesc(ptr(q), ptr(k), ptr(q_weight), ptr(k_weight), ptr(positions), ptr(inv_freq), ptr(q_out), ptr(k_out), ptr(gq),
-                      ptr(gk), ptr(dqw), ptr(dkw), None, 0, *_strides(q), *_strides(k), *_strides(q_out), *_strides(k_out),
-                      *(z if gq is None else _strides(gq)), *(z if gk is None else _strides(gk)), pos_stride, B, L, H, k.shape[2], D,
-                      2 * inv_freq.numel(), _TYPE[q.dtype], bool(interleaved), _INT_BYTES[positions.dtype], eps)
+    ps = positions.shape
+    if not (ks[0] == B and ks[1] == L and ks[3] == D and H > 0 and ks[2] > 0 and 8 <= D <= 256 and D % 8 == 0 and q_weight.shape == (D,)
+            and k_weight.shape == (D,) and (ps == (B, L) or ps == (L,)) and 2 <= 2 * inv_freq.numel() <= D and 0.0 <= eps < math.inf):
+        _rope_refuse(what, q, k, q_weight, k_weight, positions, inv_freq, eps)
+    return B, L, H, ks[2], D
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
@@ -815,86 +827,111 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
     multiple of 8 up to 256) divided by its root mean square (eps inside the root), times its weight (f32 [D]), then its first
     R = 2 len(inv_freq) dims rotated by positions * inv_freq: pairs (i, R/2 + i), or (2i, 2i + 1) with interleaved.
     positions int32 / int64 [B, L] or [L]; inv_freq f32; the angles are formed in 64 bits, all else in f32 with one rounding."""
-    q, k, q_weight, k_weight, positions, inv_freq = _rope_args("qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, eps)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    d = _rope_desc(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, eps, interleaved)
-    _call_on("lrce_qk_norm_rope_fwd", q, ctypes.byref(d), stream_of(q))
+    B, L, H, Hk, D = _rope_args("qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, eps)
+    q, *qs = _head_rows(q)
+    k, *ks = _head_rows(k)
+    q_weight, k_weight, positions, inv_freq = q_weight.contiguous(), k_weight.contiguous(), positions.contiguous(), inv_freq.contiguous()
+    q_out = q.new_empty((B, L, H, D))
+    k_out = q.new_empty((B, L, Hk, D))
+    _call_on("lrce_qk_norm_rope_fwd", q, _ROPE_PACK(
+        q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
+        k_out.data_ptr(), 0, 0, 0, 0, 0, 0, *qs, *ks, L * H * D, H * D, D, L * Hk * D, Hk * D, D, 0, 0, 0, 0, 0, 0,
+        L if positions.dim() == 2 else 0, B, L, H, Hk, D, 2 * inv_freq.numel(), _TYPE[q.dtype], bool(interleaved),
+        _INT_BYTES[positions.dtype], eps))
     return q_out, k_out
 
 
 def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """(dq, dk, dq_weight, dk_weight) of qk_norm_rope() for the gradients of its outputs; the other arguments as there.  The
     weights' gradients (f32) are summed in a fixed order."""
-    what = "qk_norm_rope_bwd"
-    q, k, q_weight, k_weight, positions, inv_freq = _rope_args(what, q, k, q_weight, k_weight, positions, inv_freq, eps)
-    for name, g, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
-        _chk(g, q.dtype, f"{what}: {name}")
-        if g.shape != x.shape or g.device != q.device:
-            raise N.NativeError(f"{what}: {name} must be {tuple(x.shape)} on {q.device}, got {tuple(g.shape)} on {g.device}")
-    dq_out, dk_out = _last1(dq_out), _last1(dk_out)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dqw = torch.empty_like(q_weight)
-    dkw = torch.empty_like(k_weight)
-    d = _rope_desc(q, k, q_weight, k_weight, positions, inv_freq, dq, dk, eps, interleaved, dq_out, dk_out, dqw, dkw)
-    n = N.lib().lrce_qk_norm_rope_bwd_workspace(ctypes.byref(d))
-    ws = torch.empty(max(n, 0), dtype=F32, device=q.device)
-    d.workspace, d.workspace_elems = ptr(ws), n
-    _call_on("lrce_qk_norm_rope_bwd", q, ctypes.byref(d), stream_of(q))
+    B, L, H, Hk, D = _rope_args("qk_norm_rope_bwd", q, k, q_weight, k_weight, positions, inv_freq, eps)
+    if not (dq_out.dtype is q.dtype and dk_out.dtype is q.dtype and dq_out.shape == q.shape and dk_out.shape == k.shape
+            and dq_out.get_device() == dk_out.get_device() == q.get_device()):
+        raise N.NativeError("qk_norm_rope_bwd: " + ", ".join(f"{n} {tuple(t.shape)} {t.dtype} on {t.device}" for n, t in (
+            ("dq_out", dq_out), ("dk_out", dk_out), ("q", q), ("k", k))))
+    q, *qs = _head_rows(q)
+    k, *ks = _head_rows(k)
+    dq_out, *gqs = _head_rows(dq_out)
+    dk_out, *gks = _head_rows(dk_out)
+    q_weight, k_weight, positions, inv_freq = q_weight.contiguous(), k_weight.contiguous(), positions.contiguous(), inv_freq.contiguous()
+    dq = q.new_empty((B, L, H, D))
+    dk = q.new_empty((B, L, Hk, D))
+    dqw = q.new_empty(D, dtype=F32)
+    dkw = q.new_empty(D, dtype=F32)
+    n = _rope_ws(B * L, D)
+    ws = q.new_empty(n, dtype=F32)
+    _call_on("lrce_qk_norm_rope_bwd", q, _ROPE_PACK(
+        q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), dq.data_ptr(),
+        dk.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(), n, *qs, *ks, L * H * D, H * D, D, L * Hk * D,
+        Hk * D, D, *gqs, *gks, L if positions.dim() == 2 else 0, B, L, H, Hk, D, 2 * inv_freq.numel(), _TYPE[q.dtype], bool(interleaved),
+        _INT_BYTES[positions.dtype], eps))
     return dq, dk, dqw, dkw
+
+
+@functools.lru_cache(maxsize=4096)
+def _rope_ws(tokens, D):
+    return N.lib().lrce_qk_norm_rope_bwd_workspace(tokens, D)
 
 
 # ---- embedding lookup and its gradient by sorted tokens (csrc/embedding.hip) -------------------------
 def _embed_ids(what, ids, dev):
-    _chk(ids, None, f"{what}: ids")
-    if ids.dtype not in _INT_BYTES or ids.device != dev:
-        raise N.NativeError(f"{what}: ids must be int32 or int64 on {dev}, got {ids.dtype} on {ids.device}")
+    if not (ids.is_cuda and ids.dtype in _INT_BYTES and ids.get_device() == dev):
+        _chk(ids, None, f"{what}: ids")
+        raise N.NativeError(f"{what}: ids must be int32 or int64 on cuda:{dev}, got {ids.dtype} on {ids.device}")
     return ids.contiguous()
 
 
 def embedding(ids, weight, scale=1.0, out_dtype=None):
     """scale * weight[ids]: ids (any shape) int32 / int64, weight [rows, cols] bf16, fp16 or f32 (rows may be strided); the result
     has weight's type, or out_dtype where weight is f32.  An id outside the table gives a row of NaN (no host check)."""
-    _chk(weight, None, "embedding: weight")
     out_dtype = weight.dtype if out_dtype is None else out_dtype
-    if weight.dim() != 2 or weight.dtype not in _TYPE or out_dtype not in _TYPE or (weight.dtype != F32 and out_dtype != weight.dtype):
+    if not (weight.is_cuda and weight.dim() == 2 and weight.dtype in _TYPE and out_dtype in _TYPE
+            and (weight.dtype is F32 or out_dtype is weight.dtype) and weight.shape[0] > 0 and weight.shape[1] > 0):
+        _chk(weight, None, "embedding: weight")
         raise N.NativeError(f"embedding: weight [rows, cols] of bf16, fp16 or f32, got {tuple(weight.shape)} {weight.dtype} -> {out_dtype}")
-    if weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise N.NativeError(f"embedding: an empty table {tuple(weight.shape)}")
-    ids = _embed_ids("embedding", ids, weight.device)
-    if weight.shape[1] > 1 and weight.stride(1) != 1 or weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]:
-        weight = weight.contiguous()
+    ids = _embed_ids("embedding", ids, weight.get_device())
     rows, cols = weight.shape
-    y = torch.empty((*ids.shape, cols), dtype=out_dtype, device=weight.device)
-    _call_on("lrce_embedding_fwd", y, ptr(ids), _INT_BYTES[ids.dtype], ids.numel(), ptr(weight), weight.stride(0) if rows > 1 else cols, rows,
-             cols, _TYPE[weight.dtype], ptr(y), _TYPE[out_dtype], float(scale), stream_of(y))
+    if weight.is_contiguous():
+        ld = cols
+    elif (cols == 1 or weight.stride(1) == 1) and weight.stride(0) >= cols:
+        ld = weight.stride(0)
+    else:
+        weight, ld = weight.contiguous(), cols
+    y = weight.new_empty((*ids.shape, cols), dtype=out_dtype)
+    _call_on("lrce_embedding_fwd", y, ids.data_ptr(), _INT_BYTES[ids.dtype], ids.numel(), weight.data_ptr(), ld, rows, cols,
+             _TYPE[weight.dtype], y.data_ptr(), _TYPE[out_dtype], scale)
     return y
+
+
+@functools.lru_cache(maxsize=4096)
+def _embed_ws(n, rows, cols):
+    return N.lib().lrce_embedding_bwd_workspace(n, rows, cols)
 
 
 def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=-1, dw=None):
     """The gradient of embedding()'s table for dy [*ids.shape, cols] (bf16, fp16 or f32): f32 [rows, cols], row v = scale * the sum
     of dy over the places where ids is v, in their order (the same bits each time); padding_idx (-1: none) and ids outside the
     table have none.  dw: a contiguous f32 [rows, cols] the gradient is added to (and returned) instead of a new tensor."""
-    _chk(dy, None, "embedding_bwd: dy")
-    if dy.dtype not in _TYPE:
+    if not (dy.is_cuda and dy.dtype in _TYPE):
+        _chk(dy, None, "embedding_bwd: dy")
         raise N.NativeError(f"embedding_bwd: dy must be bf16, fp16 or f32, got {dy.dtype}")
-    ids = _embed_ids("embedding_bwd", ids, dy.device)
-    if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] < 1 or rows < 1:
+    ids = _embed_ids("embedding_bwd", ids, dy.get_device())
+    if not (dy.shape[:-1] == ids.shape and dy.dim() == ids.dim() + 1 and dy.shape[-1] > 0 and rows > 0):
         raise N.NativeError(f"embedding_bwd: dy {tuple(dy.shape)} for ids {tuple(ids.shape)} and {rows} rows")
     cols, n = dy.shape[-1], ids.numel()
     dy = dy.contiguous()
     add = dw is not None
-    if add:
-        _chk(dw, F32, "embedding_bwd: dw")
-        if dw.shape != (rows, cols) or not dw.is_contiguous() or dw.device != dy.device or dw.data_ptr() % 16:
-            raise N.NativeError(f"embedding_bwd: dw must be a contiguous f32 {(rows, cols)} on {dy.device}")
-    else:
-        dw = torch.empty((rows, cols), dtype=F32, device=dy.device)
-    k = N.lib().lrce_embedding_bwd_workspace(n, rows, cols)
-    ws = torch.empty(max(k, 0), dtype=F32, device=dy.device)
-    _call_on("lrce_embedding_bwd", dw, ptr(ids), _INT_BYTES[ids.dtype], n, ptr(dy), _TYPE[dy.dtype], ptr(dw), rows, cols, float(scale),
-             int(padding_idx), int(add), ptr(ws), k, stream_of(dw))
+    if not add:
+        dw = dy.new_empty((rows, cols), dtype=F32)
+    elif not (dw.dtype is F32 and dw.shape == (rows, cols) and dw.is_contiguous() and dw.get_device() == dy.get_device()
+              and dw.data_ptr() % 16 == 0):
+        raise N.NativeError(f"embedding_bwd: dw must be a contiguous f32 {(rows, cols)} on {dy.device} at a multiple of 16 bytes")
+    k = _embed_ws(n, rows, cols)
+    if k < 0:
+        raise N.NativeError(f"embedding_bwd: {n} tokens of {rows} rows: too many")
+    ws = dy.new_empty(k, dtype=F32)
+    _call_on("lrce_embedding_bwd", dw, ids.data_ptr(), _INT_BYTES[ids.dtype], n, dy.data_ptr(), _TYPE[dy.dtype], dw.data_ptr(), rows, cols,
+             scale, padding_idx, add, ws.data_ptr(), k)
     return dw
 
 
