@@ -126,7 +126,7 @@ def test_norm_rope_zero_rows_and_alignment():
 
 
 # --------------------------------------------------------------------------------------------- embedding
-@pytest.mark.parametrize("N,V,C", [(1, 5, 8), (17, 30, 1000), (320, 30522, 768), (1025, 7, 96), (8192, 4000, 33), (8193, 511, 64), (20011, 128000, 40),
+@pytest.mark.parametrize("N,V,C", [(1, 5, 8), (17, 30, 1000), (320, 30522, 768), (512, 1, 4400), (512, 700, 9), (513, 700, 9), (1025, 7, 96), (8192, 4000, 33), (8193, 511, 64), (20011, 128000, 40),
                                    (40000, 3, 24)])
 @pytest.mark.parametrize("types", [("f32", "f32", "f32"), ("bf16", "bf16", "bf16"), ("f16", "f16", "f32"), ("f32", "bf16", "f16")],
                          ids=lambda t: "-".join(t))
@@ -134,9 +134,10 @@ def test_embedding(N, V, C, types):
     g = torch.Generator(device=dev).manual_seed(N)
     w = torch.randn(V, C, generator=g, device=dev).to(DT[types[0]])
     ids = (V ** torch.rand(N, generator=g, device=dev, dtype=F64)).long().clamp_(0, V - 1)
-    ids[torch.rand(N, generator=g, device=dev) < 0.3] = 1     # a frequent one
+    often = min(1, V - 1)
+    ids[torch.rand(N, generator=g, device=dev) < 0.3] = often
     dy = torch.randn(N, C, generator=g, device=dev).to(DT[types[2]])
-    for it, pad, scale in ((torch.int64, -1, 1.0), (torch.int32, 1, 27.7)):
+    for it, pad, scale in ((torch.int64, -1, 1.0), (torch.int32, often, 27.7)):
         i = ids.to(it)
         y = K().embedding(i, w, scale=scale, out_dtype=DT[types[1]])
         assert torch.equal(y, (w[ids].float() * scale).to(DT[types[1]]))

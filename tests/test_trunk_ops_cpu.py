@@ -111,10 +111,10 @@ def test_embedding_refusals():
         return L.lrce_embedding_bwd(a["ids"], a["ib"], a["n"], a["dy"], a["dt"], a["dw"], a["rows"], a["cols"], 1.0, -1, 1, a["ws"], a["k"], None)
 
     for o, word in ((dict(ib=1), b"ids"), (dict(n=1 << 31), b"sizes"), (dict(dt=5), b"type"), (dict(dw=A + 4), b"16 bytes"), (dict(dw=None), b"16 bytes"),
-                    (dict(dy=None), b"null"), (dict(), b"workspace"), (dict(ws=A + 4, k=1 << 20), b"workspace")):
+                    (dict(dy=None), b"null"), (dict(n=4000), b"workspace"), (dict(n=4000, ws=A + 4, k=1 << 20), b"workspace")):
         assert bwd(**o) == 1 and word in L.lrce_last_error(), (o, L.lrce_last_error())
     assert bwd(n=0) == 0
-    assert L.lrce_embedding_bwd_workspace(-1, 10, 16) == -1 and L.lrce_embedding_bwd_workspace(100, 10, 16) > 0
+    assert L.lrce_embedding_bwd_workspace(-1, 10, 16) == -1 and L.lrce_embedding_bwd_workspace(4000, 10, 16) > 0
 
 
 def test_wrappers_refuse_cpu_tensors():

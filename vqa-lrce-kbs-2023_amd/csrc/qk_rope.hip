@@ -125,7 +125,7 @@ struct Pairs {
 
 // NCH chunks of VEC pairs a lane (2 only where VEC = 1 and D > 128)
 template <typename T, int VEC, int NCH, bool BWD>
-__global__ void __launch_bounds__(256) qk_rope_kernel(RopeP p) {
+__global__ void __launch_bounds__(256, BWD ? 3 : 5) qk_rope_kernel(RopeP p) {
   constexpr int W = 2 * VEC;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lanes = 1 << p.lgrp, ngrp = 64 >> p.lgrp, grp = lane >> p.lgrp, li = lane & (lanes - 1);
@@ -257,21 +257,24 @@ __global__ void __launch_bounds__(256) qk_rope_kernel(RopeP p) {
   }
 }
 
-// dw[e] = the workgroups' sums in order: 16 columns a workgroup, 16 threads a column
-__global__ void __launch_bounds__(256) qk_rope_dw_kernel(RopeP p) {
-  __shared__ float red[16][17];
+// dw[e] = the workgroups' sums, 16 columns a workgroup, 64 threads a column that each add every 64th in order
+__global__ void __launch_bounds__(1024) qk_rope_dw_kernel(RopeP p) {
+  __shared__ float red[64][17];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
   float s = 0.f;
-  if (e < 2 * p.D)
-    for (int i = r; i < p.nwg; i += 16) s += p.part[(long long)i * 2 * p.D + e];
+  if (e < 2 * p.D) {
+#pragma unroll 8
+    for (int i = r; i < p.nwg; i += 64) s += p.part[(long long)i * 2 * p.D + e];
+  }
   red[r][c] = s;
   __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if (r < o) red[r][c] += red[r + o][c];
+    __syncthreads();
+  }
   if (r == 0 && e < 2 * p.D) {
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += red[i][c];
-    if (e < p.D) p.dqw[e] = s;
-    else p.dkw[e - p.D] = s;
+    if (e < p.D) p.dqw[e] = red[0][c];
+    else p.dkw[e - p.D] = red[0][c];
   }
 }
 
@@ -292,8 +295,8 @@ int rope_check(const LrceRopeDesc* d, bool bwd, const char* what) {
   return LRCE_OK;
 }
 
-// The backward leaves a row of partial sums a workgroup, four waves of at least a token each: up to 4 workgroups a CU
-int64_t rope_wgs(int64_t tokens) { return std::max<int64_t>(1, std::min<int64_t>((tokens + 3) / 4, 1024)); }
+// The backward leaves a row of partial sums a workgroup, four waves of at least a token each: up to the 3 workgroups a CU that are resident
+int64_t rope_wgs(int64_t tokens) { return std::max<int64_t>(1, std::min<int64_t>((tokens + 3) / 4, 768)); }
 
 struct RopePlan { int vec, lgrp, gpt, tpw; };
 
@@ -387,6 +390,6 @@ extern "C" int lrce_qk_norm_rope_bwd(const LrceRopeDesc* d, void* stream) {
     return lrce_fail(LRCE_E_ARG, "qk_norm_rope_bwd: a workspace of %lld floats is needed", (long long)p.nwg * 2 * d->D);
   hipStream_t s = static_cast<hipStream_t>(stream);
   rope_type<true>(p, d->dtype, f.vec, p.nwg, s);
-  qk_rope_dw_kernel<<<(2 * d->D + 15) / 16, 256, 0, s>>>(p);
+  qk_rope_dw_kernel<<<(2 * d->D + 15) / 16, 1024, 0, s>>>(p);
   return lrce_check_launch("qk_norm_rope_bwd");
 }
