@@ -21,7 +21,7 @@
 
 namespace {
 
-// One query tile (32 rows) against key blocks of 32: the state of a wave
+// One query tile (32 rows): the state of a wave
 template <int D, bool F16>
 struct FwdState {
   bf16x8 q[D / 16];
@@ -31,6 +31,7 @@ struct FwdState {
   __device__ __forceinline__ void init(const bf16* row, int h) {
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) q[kk] = *reinterpret_cast<const bf16x8*>(row + 16 * kk + 8 * h);
+    attn_landed(q);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -38,31 +39,32 @@ struct FwdState {
     m = -INFINITY;
     l = 0.f;
   }
-
-  // NKB blocks of 32 keys; kw[blk] (masked): bit = key of the block this lane's query may see, shifted by 4 h
+  // raw scores of the 32 keys from row r0 of the tile on
+  __device__ __forceinline__ f32x16 scores(const TileRead<D>& rd, lds_cptr kt, int r0) const {
+    f32x16 s = mfma32x32x16<F16>(rd.row(kt, r0, 0), q[0], f32x16{});
+#pragma unroll
+    for (int kk = 1; kk < D / 16; ++kk) s = mfma32x32x16<F16>(rd.row(kt, r0, kk), q[kk], s);
+    return s;
+  }
+  // kw[blk]: bit = key of the block this lane's query may see, shifted by 4 h
   template <int NKB>
-  __device__ __forceinline__ void tile(const TileRead<D>& rd, lds_cptr kt, lds_cptr vt, bool masked, const uint32_t* kw, float c) {
-    f32x16 s[NKB];
+  __device__ __forceinline__ static void hide(f32x16 (&s)[NKB], const uint32_t* kw) {
 #pragma unroll
-    for (int blk = 0; blk < NKB; ++blk) {
+    for (int blk = 0; blk < NKB; ++blk)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[blk][r] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) s[blk] = mfma32x32x16<F16>(rd.row(kt, 32 * blk, kk), q[kk], s[blk]);
-    }
-    if (masked) {
-#pragma unroll
-      for (int blk = 0; blk < NKB; ++blk)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[blk][r] = (kw[blk] >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[blk][r] : -INFINITY;
-    }
+      for (int r = 0; r < 16; ++r) s[blk][r] = (kw[blk] >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[blk][r] : -INFINITY;
+  }
+  template <int NKB>
+  __device__ __forceinline__ static float top(const f32x16 (&s)[NKB]) {
     float mx = s[0][0];
 #pragma unroll
     for (int blk = 0; blk < NKB; ++blk)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[blk][r]);
-    mx = fmaxf(mx, other_half(mx));
+    return fmaxf(mx, other_half(mx));
+  }
+  // the running maximum follows mx where it has to
+  __device__ __forceinline__ void raise(float mx, float c) {
     if (__any(mx > m && !((mx - m) * c <= 8.f))) {
       const float mn = fmaxf(m, mx);
       const float a = mn > m ? __builtin_amdgcn_exp2f((m - mn) * c) : 1.f;
@@ -73,41 +75,49 @@ struct FwdState {
         for (int r = 0; r < 16; ++r) acc[i][r] *= a;
       m = mn;
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
-    float t = 0.f;
+  }
+  __device__ __forceinline__ float offset(float c) const { return m == -INFINITY ? 0.f : m * c; }
+  // scores -> weights (16 bits), their sum
+  __device__ __forceinline__ void weigh(f32x16& s, bf16x8 (&pf)[2], float c, float mc) {
+    float t[4] = {l, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int blk = 0; blk < NKB; ++blk)
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[blk][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[blk][r], c, -mc));
-        t += s[blk][r];
+      for (int r = 8 * half; r < 8 * half + 8; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mc));
+        t[r & 3] += s[r];
       }
-    l += t;
+      pf[half] = attn_pack<F16>(s, half);
+    }
+    l = (t[0] + t[1]) + (t[2] + t[3]);
+  }
+  // the 32 keys from row r0 of the tile on
+  __device__ __forceinline__ void sum(const TileRead<D>& rd, lds_cptr vt, int r0, const bf16x8 (&pf)[2]) {
 #pragma unroll
-    for (int blk = 0; blk < NKB; ++blk)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const bf16x8 pf = attn_pack<F16>(s[blk], half);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] = mfma32x32x16<F16>(rd.col(vt, 32 * blk + 16 * half, i), pf, acc[i]);
-      }
+      for (int i = 0; i < D / 32; ++i) acc[i] = mfma32x32x16<F16>(rd.col(vt, r0 + 16 * k, i), pf[k], acc[i]);
   }
 };
 
-template <int D, bool F16, int NW>
+// Pipelined by one tile: the scores of the next tile (matrix pipe) are formed while the current one is exponentiated, its
+// maximum while the current one is multiplied by V.  So K runs one tile ahead of V in LDS, two places each.
+template <int D, bool F16, int NW, bool MASK>
 __global__ void __launch_bounds__(NW * 64, 2) attn_fwd_kernel(AttnP p) {
   constexpr int KT = 64, TB = KT * D * 2;
   typedef TileStage<D, KT, NW> Stage;
-  __shared__ __attribute__((aligned(1024))) char buf[4 * TB];            // K, V of two tiles
-  __shared__ uint64_t words[ATTN_MASK_KEYS / KT];
+  __shared__ __attribute__((aligned(1024))) char buf[4 * TB];            // K, K, V, V
+  __shared__ uint64_t words[MASK ? ATTN_MASK_KEYS / KT : 1];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int blk = p.nblk - 1 - id % p.nblk, bh = id / p.nblk, b = bh / p.H, hq = bh % p.H, hk = hq / p.G;
+  const Place at = attn_place(p, p.G);
+  const int blk = p.nblk - 1 - at.blk, b = at.b, hq = at.hq, hk = hq / p.G, bh = b * p.H + hq;   // (causal: the last rows see most)
   const int i0 = blk * (32 * NW) + wave * 32;                            // this wave's first row
   const int row = min(i0 + (lane & 31), p.Lq - 1);
   const int last = min(blk * (32 * NW) + 32 * NW, p.Lq) - 1;             // the workgroup's last row
   const int nk = p.causal ? max(0, min(p.Lk, last + p.off + 1)) : p.Lk;
   const int nt = (nk + KT - 1) / KT;
+  // tiles from tw on hold no key that this wave's rows see
+  const int tw = p.causal ? min(nt, max(0, i0 + 31 + p.off + KT) / KT) : nt;
 
   FwdState<D, F16> st;
   st.init(p.q + b * p.sqb + row * p.sql + hq * p.sqh, h);
@@ -118,53 +128,107 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_fwd_kernel(AttnP p) {
   sv.init(lane, wave, p.svl);
   const char* kb = uni(p.k + b * p.skb + hk * p.skh);
   const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  const long long kstep = p.skl * (2 * KT), vstep = p.svl * (2 * KT);
   lds_ptr lds = (lds_ptr)buf;
   LRCE_LDS uint64_t* lw = (LRCE_LDS uint64_t*)words;
 
-  const int chunk = p.mask ? ATTN_MASK_KEYS / KT : nt;
+  const int chunk = MASK ? ATTN_MASK_KEYS / KT : nt;
   for (int c0 = 0; c0 < nt; c0 += chunk) {
     const int c1 = min(nt, c0 + chunk);
-    if (p.mask) {
+    if constexpr (MASK) {
       __syncthreads();
       attn_pack_mask<NW>(p, b, c0, c1 - c0, lw, lane, wave);
       __syncthreads();
     }
-    auto word = [&](int t) { return p.mask ? uni64(lw[t - c0]) : low_bits(p.Lk - t * KT); };
     auto next = [&](int t, uint64_t& w) {      // the first tile from t on with a visible key
-      for (; t < c1; ++t)
-        if ((w = word(t)) != 0) break;
+      if constexpr (MASK) {
+        for (; t < c1; ++t)
+          if ((w = uni64(lw[t - c0])) != 0) break;
+      } else {
+        w = low_bits(p.Lk - t * KT);
+      }
       return t;
     };
-    auto stage = [&](int t, uint64_t w, int cur) {
-      const bool all = w == ~0ull;
-      sk.load(kb + (long long)t * KT * p.skl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + 2 * cur * TB), wave);
-      sv.load(vb + (long long)t * KT * p.svl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + (2 * cur + 1) * TB), wave);
+    auto stage = [&](const Stage& s, const char* base, long long step, int t, uint64_t w, int at) {
+      const uint32_t dst = attn_lds_u32(lds + at * TB);
+      if (MASK && w != ~0ull) s.load(base + t * step, p.Lk - t * KT, w, dst, lane, wave);
+      else s.load(base + t * step, p.Lk - t * KT, dst, wave);
     };
-    uint64_t w = 0, wn = 0;
-    int t = next(c0, w), cur = 0;
-    if (t < c1) stage(t, w, 0);
-    while (t < c1) {
-      attn_barrier();
-      const int tn = next(t + 1, wn);
-      if (tn < c1) stage(tn, wn, cur ^ 1);
-      const int j0 = t * KT;
-      const int lim = i0 + p.off - j0;                                     // the wave's first row sees keys up to j0 + lim
-      if (!p.causal || lim + 31 >= 0) {
-        const bool diag = p.causal && lim < KT - 1;
-        const bool masked = diag || w != ~0ull;
-        uint32_t kw[2];
-        if (masked) {
-          const int mine = lim + (lane & 31);
-          kw[0] = (uint32_t)w & (diag ? upto(mine) : ~0u);
-          kw[1] = (uint32_t)(w >> 32) & (diag ? upto(mine - 32) : ~0u);
-          kw[0] >>= 4 * h;
-          kw[1] >>= 4 * h;
-        }
-        st.template tile<2>(rd, lds + 2 * cur * TB, lds + (2 * cur + 1) * TB, masked, kw, p.c);
+    f32x16 s[2];
+    float mx;
+    auto mask = [&](int t, uint64_t w, f32x16 (&x)[2]) {
+      const int lim = i0 + p.off - t * KT;                               // the wave's first row sees keys up to t KT + lim
+      const bool diag = p.causal && lim < KT - 1;
+      if (diag || w != ~0ull) {
+        const int mine = lim + (lane & 31);
+        const uint32_t kw[2] = {((uint32_t)w & (diag ? upto(mine) : ~0u)) >> (4 * h),
+                                ((uint32_t)(w >> 32) & (diag ? upto(mine - 32) : ~0u)) >> (4 * h)};
+        st.template hide<2>(x, kw);
       }
-      t = tn;
-      w = wn;
+    };
+    uint64_t w = 0, w1 = 0, w2 = 0;
+    int t = next(c0, w);
+    if (t >= c1) continue;
+    stage(sk, kb, kstep, t, w, 0);
+    int t1 = next(t + 1, w1), cur = 0;
+    attn_barrier();
+    if (t1 < c1) stage(sk, kb, kstep, t1, w1, 1);
+    stage(sv, vb, vstep, t, w, 2);
+    if (t < tw) {
+      s[0] = st.scores(rd, lds, 0);
+      s[1] = st.scores(rd, lds, 32);
+      mask(t, w, s);
+      mx = st.template top<2>(s);
+    }
+    // a step: K of t1 and V of t are there, K of t and V before it are done with; the tiles after them are sent for
+    auto step = [&] {
+      attn_barrier();
+      const int t2 = next(t1 + 1, w2);
+      if (t2 < c1) stage(sk, kb, kstep, t2, w2, cur);
+      if (t1 < c1) stage(sv, vb, vstep, t1, w1, 2 + (cur ^ 1));
+      return t2;
+    };
+    int t2 = step();
+    while (t1 < c1 && t1 < tw) {
+      bf16x8 p0[2], p1[2];
+      st.raise(mx, p.c);
+      const float mc = st.offset(p.c);
+      lds_cptr kt = lds + (cur ^ 1) * TB, vt = lds + (2 + cur) * TB;
+      f32x16 sn[2];
+      __builtin_amdgcn_sched_barrier(0);
+      sn[0] = st.scores(rd, kt, 0);
+      st.weigh(s[0], p0, p.c, mc);
+      attn_interleave<D / 16, 128 / D * 7>();
+      __builtin_amdgcn_sched_barrier(0);
+      sn[1] = st.scores(rd, kt, 32);
+      st.sum(rd, vt, 0, p0);
+      st.weigh(s[1], p1, p.c, mc);
+      attn_interleave<D / 8, 128 / D * 4>();
+      __builtin_amdgcn_sched_barrier(0);
+      st.sum(rd, vt, 32, p1);
+      mask(t1, w1, sn);
+      mx = st.template top<2>(sn);
+      s[0] = sn[0];
+      s[1] = sn[1];
+      t = t1; w = w1; t1 = t2; w1 = w2;
       cur ^= 1;
+      t2 = step();
+    }
+    if (t < tw) {                                                        // this wave's last tile
+      bf16x8 pf[2];
+      st.raise(mx, p.c);
+      const float mc = st.offset(p.c);
+      lds_cptr vt = lds + (2 + cur) * TB;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        st.weigh(s[blk], pf, p.c, mc);
+        st.sum(rd, vt, 32 * blk, pf);
+      }
+    }
+    while (t1 < c1) {                                                    // the other waves' steps
+      t1 = t2; w1 = w2;
+      cur ^= 1;
+      t2 = step();
     }
   }
   const float l = st.l + other_half(st.l);
@@ -206,6 +270,7 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP 
   sv.init(lane, 0, p.svl);
   const char* kb = uni(p.k + b * p.skb + hk * p.skh);
   const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  const long long kstep = p.skl * (2 * KT), vstep = p.svl * (2 * KT);
   lds_ptr lds = (lds_ptr)buf + wave * (NST * 2 * TB);
   LRCE_LDS uint64_t* lw = (LRCE_LDS uint64_t*)words;
 
@@ -226,9 +291,16 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP 
       return t;
     };
     auto stage = [&](int t, uint32_t w, int cur) {
-      const bool all = w == ~0u;
-      sk.load(kb + (long long)t * KT * p.skl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + 2 * cur * TB), 0);
-      sv.load(vb + (long long)t * KT * p.svl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + (2 * cur + 1) * TB), 0);
+      const char *ka = kb + t * kstep, *va = vb + t * vstep;
+      const uint32_t kd = attn_lds_u32(lds + 2 * cur * TB), vd = attn_lds_u32(lds + (2 * cur + 1) * TB);
+      const int n = p.Lk - t * KT;
+      if (p.mask && w != ~0u) {
+        sk.load(ka, n, w, kd, lane, 0);
+        sv.load(va, n, w, vd, lane, 0);
+      } else {
+        sk.load(ka, n, kd, 0);
+        sv.load(va, n, vd, 0);
+      }
     };
     uint32_t w0 = 0, w1 = 0, w2 = 0;
     int cur = 0;
@@ -241,8 +313,16 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP 
       else attn_wait_vm<0>();
       const int lim = p.causal ? qi + p.off - t0 * KT : 31;
       const bool masked = w0 != ~0u || (p.causal && __any(lim < 31));
-      uint32_t kw[1] = {(w0 & upto(lim)) >> (4 * h)};
-      st.template tile<1>(rd, lds + 2 * cur * TB, lds + (2 * cur + 1) * TB, masked, kw, p.c);
+      f32x16 s[1];
+      bf16x8 pf[2];
+      s[0] = st.scores(rd, lds + 2 * cur * TB, 0);
+      if (masked) {
+        const uint32_t kw[1] = {(w0 & upto(lim)) >> (4 * h)};
+        st.template hide<1>(s, kw);
+      }
+      st.raise(st.template top<1>(s), p.c);
+      st.weigh(s[0], pf, p.c, st.offset(p.c));
+      st.sum(rd, lds + (2 * cur + 1) * TB, 0, pf);
       const int t2 = next(t1 + NW, w2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the tile's reads are done: its place may be filled
       if (t2 < c1) stage(t2, w2, cur);
@@ -426,9 +506,11 @@ void fwd_launch(const AttnP& p, const FwdPlan& f, hipStream_t s) {
       attn_join_kernel<D, F16><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(p);
     }
   } else if (f.waves == 2) {
-    attn_fwd_kernel<D, F16, 2><<<(unsigned)f.grid, 128, 0, s>>>(p);
+    if (p.mask) attn_fwd_kernel<D, F16, 2, true><<<(unsigned)f.grid, 128, 0, s>>>(p);
+    else attn_fwd_kernel<D, F16, 2, false><<<(unsigned)f.grid, 128, 0, s>>>(p);
   } else {
-    attn_fwd_kernel<D, F16, 4><<<(unsigned)f.grid, 256, 0, s>>>(p);
+    if (p.mask) attn_fwd_kernel<D, F16, 4, true><<<(unsigned)f.grid, 256, 0, s>>>(p);
+    else attn_fwd_kernel<D, F16, 4, false><<<(unsigned)f.grid, 256, 0, s>>>(p);
   }
 }
 

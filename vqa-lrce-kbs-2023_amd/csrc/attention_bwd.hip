@@ -21,8 +21,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
   __shared__ __attribute__((aligned(1024))) char buf[4 * TB];
   __shared__ uint64_t words[ATTN_MASK_KEYS / KT];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int blk = p.nblk - 1 - id % p.nblk, bh = id / p.nblk, b = bh / p.H, hq = bh % p.H, hk = hq / p.G;
+  const Place at = attn_place(p, p.G);
+  const int blk = p.nblk - 1 - at.blk, b = at.b, hq = at.hq, hk = hq / p.G, bh = b * p.H + hq;
   const int i0 = blk * (32 * NW) + wave * 32;
   const bool valid = i0 + n < p.Lq;
   const int row = min(i0 + n, p.Lq - 1);
@@ -45,6 +45,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
       for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(from16<F16>(g[kk][j]), from16<F16>(o[j]), delta);
     }
   }
+  attn_landed(q);
+  attn_landed(g);
   delta += other_half(delta);
   const float lse = p.lse[(long long)bh * p.Lq + row];
   // a row that sees no key has lse = -inf and p = exp(s - inf) = 0; so have the rows behind the last
@@ -64,6 +66,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
   sv.init(lane, wave, p.svl);
   const char* kb = uni(p.k + b * p.skb + hk * p.skh);
   const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  const long long kstep = p.skl * (2 * KT), vstep = p.svl * (2 * KT);
   lds_ptr lds = (lds_ptr)buf;
   LRCE_LDS uint64_t* lw = (LRCE_LDS uint64_t*)words;
   const int chunk = p.mask ? ATTN_MASK_KEYS / KT : nt;
@@ -81,9 +84,16 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
       return t;
     };
     auto stage = [&](int t, uint64_t w, int cur) {
-      const bool all = w == ~0ull;
-      sk.load(kb + (long long)t * KT * p.skl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + 2 * cur * TB), wave);
-      sv.load(vb + (long long)t * KT * p.svl * 2, p.Lk - t * KT, w, all, attn_lds_u32(lds + (2 * cur + 1) * TB), wave);
+      const char *ka = kb + t * kstep, *va = vb + t * vstep;
+      const uint32_t kd = attn_lds_u32(lds + 2 * cur * TB), vd = attn_lds_u32(lds + (2 * cur + 1) * TB);
+      const int n = p.Lk - t * KT;
+      if (p.mask && w != ~0ull) {
+        sk.load(ka, n, w, kd, lane, wave);
+        sv.load(va, n, w, vd, lane, wave);
+      } else {
+        sk.load(ka, n, kd, wave);
+        sv.load(va, n, vd, wave);
+      }
     };
     uint64_t w = 0, wn = 0;
     int t = next(c0, w), cur = 0;
@@ -139,8 +149,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 96 ? 2 : 1) attn_dkv_kernel(Attn
   typedef TileStage<D, QT, NW> Stage;
   __shared__ __attribute__((aligned(1024))) char buf[4 * TB + 2 * SB];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int sp = id % p.nsplit, rest = id / p.nsplit, blk = rest % p.nblk, bk = rest / p.nblk, b = bk / p.Hk, hk = bk % p.Hk;
+  const Place place = attn_place(p, p.nsplit);                           // (the splits take the place of the group's heads)
+  const int blk = place.blk, b = place.b, hk = place.hq / p.nsplit, sp = place.hq % p.nsplit, bk = b * p.Hk + hk;
   const int j0 = blk * (32 * NW) + wave * 32, jw = blk * (32 * NW);
   const int j = j0 + n;
   bool keep = j < p.Lk;
@@ -163,6 +173,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 96 ? 2 : 1) attn_dkv_kernel(Attn
       kf[kk] = keep ? *reinterpret_cast<const bf16x8*>(kr + 16 * kk + 8 * h) : zero;
       vf[kk] = keep ? *reinterpret_cast<const bf16x8*>(vr + 16 * kk + 8 * h) : zero;
     }
+    attn_landed(kf);
+    attn_landed(vf);
   }
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -187,9 +199,12 @@ __global__ void __launch_bounds__(NW * 64, D <= 96 ? 2 : 1) attn_dkv_kernel(Attn
     const int rows = p.Lq - ts * QT;
     const char* qb = uni(p.q + b * p.sqb + hq * p.sqh + (long long)ts * QT * p.sql);
     const char* gb = uni(p.dout + b * p.sgb + hq * p.sgh + (long long)ts * QT * p.sgl);
-    sq.load(qb, rows, 0, true, attn_lds_u32(lds + 2 * cur * TB), wave);
-    sg.load(gb, rows, 0, true, attn_lds_u32(lds + (2 * cur + 1) * TB), wave);
-    if (wave == 0) attn_glds(uni(p.ws + (((long long)b * p.H + hq) * nst + 2 * ts) * 64), 512, lane * 16, attn_lds_u32(lds + 4 * TB + cur * SB));
+    sq.load(qb, rows, attn_lds_u32(lds + 2 * cur * TB), wave);
+    sg.load(gb, rows, attn_lds_u32(lds + (2 * cur + 1) * TB), wave);
+    if (wave == 0) {
+      const uint32_t o = lane * 16;
+      attn_glds<1, 0>(attn_rsrc(uni(p.ws + (((long long)b * p.H + hq) * nst + 2 * ts) * 64), 512), &o, attn_lds_u32(lds + 4 * TB + cur * SB));
+    }
     if (++ts == nq) { ts = tf; ++hs; }
   };
   int cur = 0, tc = ts;

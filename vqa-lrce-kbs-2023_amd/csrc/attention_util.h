@@ -86,6 +86,35 @@ struct TileRead {
 };
 
 __device__ __forceinline__ uint32_t attn_lds_u32(lds_cptr p) { return (uint32_t)(uintptr_t)p; }
+// Workgroup -> (head, block).  Without causality a head's blocks are neighbours on one XCD, whose L2 keeps its K and V.  With
+// it the blocks differ in work: the longest of all heads come first, and a head's workgroups stay on one XCD where the
+// number of (batch, key head) pairs allows (ids go round the 8 XCDs), query heads of a group together.
+struct Place { int b, hq, blk; };
+__device__ __forceinline__ Place attn_place(const AttnP& p, int heads_per_key) {
+  Place x;
+  if (p.causal) {
+    const int nk = p.B * p.Hk, n = nk * heads_per_key, j = blockIdx.x % n, bk = j % nk;
+    x.blk = blockIdx.x / n;
+    x.b = bk / p.Hk;
+    x.hq = (bk % p.Hk) * heads_per_key + j / nk;
+  } else {
+    const int id = xcd_remap(blockIdx.x, gridDim.x), bh = id / p.nblk, h = p.Hk * heads_per_key;
+    x.blk = id % p.nblk;
+    x.b = bh / h;
+    x.hq = bh % h;
+  }
+  return x;
+}
+
+// Scheduling: GROUPS times one matrix instruction, then VALU vector instructions (the compiler's own order clusters each kind)
+template <int GROUPS, int VALU>
+__device__ __forceinline__ void attn_interleave() {
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, VALU, 0);
+  }
+}
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ const char* uni(const void* p) {
   const uint64_t a = reinterpret_cast<uintptr_t>(p);
@@ -93,18 +122,40 @@ __device__ __forceinline__ const char* uni(const void* p) {
                                        ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32));
 }
 
-// 64 lanes x 16 bytes from base + voff (zeros where voff + 16 > bytes) to LDS at dst (wave-uniform, 1 KB).  In asm, so
-// that the compiler does not drain the loads in flight before every LDS read; the loops' own waits order them.
-__device__ __forceinline__ void attn_glds(const char* base, uint32_t bytes, uint32_t voff, uint32_t dst) {
+// A buffer of `bytes` bytes at a wave-uniform address; what lies at or past its end reads as zeros
+__device__ __forceinline__ i32x4 attn_rsrc(const char* base, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uintptr_t>(base);
   i32x4 rs;
   rs[0] = (int)(uint32_t)a;
   rs[1] = (int)(uint32_t)((a >> 32) & 0xffffu);
   rs[2] = (int)bytes;
   rs[3] = 0x00020000;
+  return rs;
+}
+// N loads of 64 lanes x 16 bytes from rs + voff[i] to LDS at dst + i * STEP (wave-uniform, 1 KB each).  In asm, so that the
+// compiler does not drain the loads in flight before every LDS read; the loops' own waits order them.
+template <int N, int STEP>
+__device__ __forceinline__ void attn_glds(i32x4 rs, const uint32_t* voff, uint32_t dst) {
   unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(voff), "s"(rs), "s"(dst) : "memory");
+  if constexpr (N >= 4) {
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\ts_add_u32 m0, m0, %7\n\t"
+                 "s_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\t"
+                 "buffer_load_dwordx4 %3, %5, 0 offen lds\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(rs), "s"(dst), "n"(STEP) : "memory", "scc");
+    attn_glds<N - 4, STEP>(rs, voff + 4, dst + 4 * STEP);
+  } else if constexpr (N >= 1) {
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff[0]), "s"(rs), "s"(dst) : "memory");
+    attn_glds<N - 1, STEP>(rs, voff + 1, dst + STEP);
+  }
+}
+// Operands that a loop with loads to LDS in flight reads from registers have to have landed before it: the compiler, which
+// does not see those loads, would else wait for every load at the operands' first use in each iteration.
+template <int N>
+__device__ __forceinline__ void attn_landed(bf16x8 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 template <int N>
 __device__ __forceinline__ void attn_wait_vm() {
@@ -115,32 +166,34 @@ __device__ __forceinline__ void attn_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// Staging of a tile [ROWS][D] by NW waves: NI loads of 1 KB each a wave
+// Staging of tiles [ROWS][D] by NW waves: NI loads of 1 KB each a wave
 template <int D, int ROWS, int NW>
 struct TileStage {
   static constexpr int CH = D / 8, NI = ROWS * CH / (64 * NW), BYTES = ROWS * D * 2;
   static_assert(NI * 64 * NW == ROWS * CH, "whole loads");
   uint32_t voff[NI];
-  int rowi[NI];
   uint32_t pitch;
+  __device__ __forceinline__ static int row_of(int i, int lane, int wave) { return ((i * NW + wave) * 64 + lane) / CH; }
   __device__ __forceinline__ void init(int lane, int wave, long long ld) {
     pitch = (uint32_t)(ld * 2);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int id = (i * NW + wave) * 64 + lane, row = id / CH, cp = id % CH;
-      rowi[i] = row;
       voff[i] = (uint32_t)row * pitch + (uint32_t)((cp ^ attn_swz<D>(row)) << 4);
     }
   }
-  // rows [0, n) of the tile at base (0 < n); keep: bit r = 0 leaves row r zero
-  __device__ __forceinline__ void load(const char* base, int n, uint64_t keep, bool all, uint32_t dst, int wave) const {
-    const uint32_t bytes = (uint32_t)(min(n, ROWS) - 1) * pitch + 2 * D;
+  // bytes of the tile's first n rows (0 < n)
+  __device__ __forceinline__ uint32_t bytes(int n) const { return (uint32_t)(min(n, ROWS) - 1) * pitch + 2 * D; }
+  // the tile at base, of which the first n rows exist
+  __device__ __forceinline__ void load(const char* base, int n, uint32_t dst, int wave) const {
+    attn_glds<NI, NW * 1024>(attn_rsrc(base, bytes(n)), voff, dst + (uint32_t)wave * 1024);
+  }
+  // the same; row r is left zero where bit r of keep is 0
+  __device__ __forceinline__ void load(const char* base, int n, uint64_t keep, uint32_t dst, int lane, int wave) const {
+    uint32_t o[NI];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      uint32_t o = voff[i];
-      if (!all) o = ((keep >> rowi[i]) & 1) ? o : 0x80000000u;
-      attn_glds(base, bytes, o, dst + (uint32_t)(i * NW + wave) * 1024);
-    }
+    for (int i = 0; i < NI; ++i) o[i] = ((keep >> row_of(i, lane, wave)) & 1) ? voff[i] : 0x80000000u;
+    attn_glds<NI, NW * 1024>(attn_rsrc(base, bytes(n)), o, dst + (uint32_t)wave * 1024);
   }
 };
 
