@@ -46,17 +46,20 @@ constexpr int ATTN_MASK_KEYS = 16384;   // keys whose mask bits lie in LDS at a 
 
 __device__ __forceinline__ int crow32(int reg, int h) { return (reg & 3) + 8 * (reg >> 2) + 4 * h; }
 
-// XOR of the 16-byte chunk index: 3 bits where a row has 8 or 16 chunks, 2 bits where it has 4 or 12
+// XOR of the 16-byte chunk index.  LDS serves 256 bytes a cycle: 16 lanes of a row read (16 rows, one chunk) and 32 lanes
+// of a transposing read (4 rows, an aligned group of 4 chunks) have to fall on the 16 chunk places of 256 bytes.  A row
+// is 16, 8, 12 or 4 chunks, so rows themselves take turns of 1, 2, 4 or 4 places; the XOR does the rest with 4, 3, 2 or 2 bits.
 template <int D>
 __device__ __forceinline__ int attn_swz(int row) {
-  if constexpr (D % 64 == 0) return ((row & 3) << 1) | ((row >> 2) & 1);
-  else return (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
+  if constexpr (D == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else if constexpr (D == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else return (row >> 2) & 3;
 }
 
 // Per-lane byte offsets of the operand reads of a tile [rows][D]
 template <int D>
 struct TileRead {
-  static constexpr int NV = D % 64 == 0 ? 4 : 2, NT = D % 64 == 0 ? 2 : 1, PITCH = 2 * D;
+  static constexpr int NV = D == 128 ? 8 : D == 64 ? 4 : 2, NT = D == 128 ? 4 : D == 64 ? 2 : 1, PITCH = 2 * D;
   int ka[NV], va[NT];
   __device__ __forceinline__ void init(int lane) {
     const int r = lane & 31, h = lane >> 5;
@@ -71,13 +74,14 @@ struct TileRead {
   __device__ __forceinline__ bf16x8 row(lds_cptr t, int r0, int kk) const {
     return *reinterpret_cast<const LRCE_LDS bf16x8*>(t + ka[kk % NV] + (kk / NV) * (NV * 32) + r0 * PITCH);
   }
-  // A[m = column 32 blk + lane & 31][k = rows r0 .. r0 + 15 in the accumulator's order]   (r0 a multiple of 16)
+  // A[m = column 32 blk + lane & 31][k = rows r0 .. r0 + 15 in the accumulator's order]   (r0 a multiple of 16).  The swizzle
+  // of row + 8 is that of row with bit 1 flipped.
   __device__ __forceinline__ bf16x8 col(lds_cptr t, int r0, int blk) const {
     bf16x8 o;
 #pragma unroll
     for (int h2 = 0; h2 < 2; ++h2) {
-      lds_cptr a = t + va[blk % NT] + (blk / NT) * (NT * 64) + (r0 + 8 * h2) * PITCH;
-      s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LRCE_LDS s16x4*)(a));
+      const int at = (va[blk % NT] + (blk / NT) * (NT * 64)) ^ (h2 * 32);
+      s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LRCE_LDS s16x4*)(t + at + (r0 + 8 * h2) * PITCH));
       const bf16x4 b = __builtin_bit_cast(bf16x4, v);
       o[4 * h2 + 0] = b[0]; o[4 * h2 + 1] = b[1]; o[4 * h2 + 2] = b[2]; o[4 * h2 + 3] = b[3];
     }
