@@ -12,8 +12,7 @@
 //
 // attn_fwd_kernel: a wave has 32 query rows, a workgroup NW waves that share K / V tiles of 64 keys, double buffered.
 // attn_split_kernel: few rows (single tokens).  All query heads of a key head are rows of one tile, so K / V are read
-// once; each wave walks 32-key tiles of its own (no barrier in the loop), the workgroup's share of the keys is joined in
-// LDS and the shares of several workgroups by attn_join_kernel.
+// once; each wave walks 32-key tiles of its own and the waves' shares of the keys are joined.
 #include <algorithm>
 #include <cmath>
 
@@ -240,20 +239,27 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_fwd_kernel(AttnP p) {
   if (valid && h == 0) p.lse[(long long)bh * p.Lq + row] = l == 0.f ? -INFINITY : st.m * p.scale + __logf(l);
 }
 
-// The rows of a key head: r = i * G + g for query i and head g of the group, 32 a tile.  A workgroup takes key tiles
-// [split * split_tiles, ...) of 32 keys, wave w every fourth of them.
-template <int D, bool F16>
-__global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP p) {
-  constexpr int NW = 4, KT = 32, TB = KT * D * 2, NST = 2;
+// What a share (maximum m, sum l) counts at the common maximum mx; a share that saw nothing counts nothing
+__device__ __forceinline__ float join_factor(float m, float l, float mx, float c) {
+  return m == -INFINITY && l == 0.f ? 0.f : l != l ? l : __builtin_amdgcn_exp2f((m - mx) * c);
+}
+
+// The rows of a key head: r = i * G + g for query i and head g of the group, 32 a tile.  A workgroup takes the key tiles
+// [split * split_tiles, ...) of 32 keys, wave w every NW-th of them; a wave has its own tiles in LDS and waits for nobody.
+// NW = 2, 4: one workgroup a row tile, the waves' shares joined in LDS.  NW = 1: long key axes, cut into shares of one wave
+// each (four to eight of them a CU: one's start and end is hidden by the others), joined by attn_join_kernel.
+template <int D, bool F16, int NW>
+__global__ void __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) attn_split_kernel(AttnP p) {
+  constexpr int KT = 32, TB = KT * D * 2, NST = 2;
   typedef TileStage<D, KT, 1> Stage;
   constexpr int OP = D + 4;                                              // padded row of a joined output tile (floats)
-  constexpr int SZ = NW * NST * 2 * TB > NW * 32 * OP * 4 ? NW * NST * 2 * TB : NW * 32 * OP * 4;
+  constexpr int SZ = NW > 1 && NW * 32 * OP * 4 > NW * NST * 2 * TB ? NW * 32 * OP * 4 : NW * NST * 2 * TB;
   __shared__ __attribute__((aligned(1024))) char buf[SZ];
-  __shared__ uint64_t words[ATTN_MASK_KEYS / 64];
   __shared__ float sm[NW][32], sl[NW][32];
-  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int sp = id % p.nsplit, rest = id / p.nsplit, rt = rest % p.nblk, bk = rest / p.nblk, b = bk / p.Hk, hk = bk % p.Hk;
+  const int lane = threadIdx.x & 63, wave = NW > 1 ? uni(threadIdx.x >> 6) : 0, h = lane >> 5, n = lane & 31;
+  // shares go round the XCDs (batch rows differ in visible keys); the row tiles of one share meet on one where their number allows
+  const int un = gridDim.x / p.nblk, id = blockIdx.x % un, rt = blockIdx.x / un;
+  const int sp = id % p.nsplit, bk = id / p.nsplit, b = bk / p.Hk, hk = bk % p.Hk;
   const int R = p.Lq * p.G;
   const int r = min(rt * 32 + n, R - 1), qi = r / p.G, hq = hk * p.G + r % p.G;
   const int last = (min(rt * 32 + 31, R - 1)) / p.G;
@@ -272,18 +278,20 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP 
   const char* vb = uni(p.v + b * p.svb + hk * p.svh);
   const long long kstep = p.skl * (2 * KT), vstep = p.svl * (2 * KT);
   lds_ptr lds = (lds_ptr)buf + wave * (NST * 2 * TB);
-  LRCE_LDS uint64_t* lw = (LRCE_LDS uint64_t*)words;
 
-  const int chunk = p.mask ? ATTN_MASK_KEYS / KT : max(b1 - b0, 1);
+  // the mask bits of 128 tiles at a time: lane l has those of keys 64 l .. 64 l + 63
+  const int chunk = p.mask ? 128 : max(b1 - b0, 1);
   for (int c0 = b0; c0 < b1; c0 += chunk) {
     const int c1 = min(b1, c0 + chunk);
-    if (p.mask) {
-      __syncthreads();
-      attn_pack_mask<NW>(p, b, c0 / 2, (c1 - c0 + 1) / 2, lw, lane, wave);
-      __syncthreads();
-    }
+    uint32_t mlo = 0, mhi = 0;
+    if (p.mask)
+      attn_mask_words<1>(p, b, c0 / 2, (c1 + 1) / 2, lane, [&](int w, uint64_t bits) {
+        if (lane == w - c0 / 2) { mlo = (uint32_t)bits; mhi = (uint32_t)(bits >> 32); }
+      });
     auto word = [&](int t) {
-      return p.mask ? (uint32_t)(uni64(lw[(t - c0) >> 1]) >> (32 * ((t - c0) & 1))) : (uint32_t)low_bits(p.Lk - t * KT);
+      if (!p.mask) return (uint32_t)low_bits(p.Lk - t * KT);
+      const int w = (t - c0) >> 1;
+      return (uint32_t)__builtin_amdgcn_readlane(((t - c0) & 1) ? mhi : mlo, w);
     };
     auto next = [&](int t, uint32_t& w) {
       for (; t < c1; t += NW)
@@ -331,41 +339,56 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP 
       cur ^= 1;
     }
   }
-  // the four waves' shares: o_w relative to m_w, joined at the common maximum
   const float l = st.l + other_half(st.l);
-  if (h == 0) { sm[wave][n] = st.m; sl[wave][n] = l; }
-  __syncthreads();
-  float* so = reinterpret_cast<float*>(buf) + wave * 32 * OP;
+  const long long rows = (long long)p.B * p.H * p.Lq;
+  if constexpr (NW == 1) {
+    // partials [split][row][D] and (maximum, sum), both before the division
+    if (rt * 32 + n < R) {
+      const long long at = (long long)sp * rows + ((long long)b * p.H + hq) * p.Lq + qi;
+      float* dst = p.ws + at * D + 4 * h;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      f32x4 x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = st.acc[i][4 * u + e];
-      *reinterpret_cast<f32x4*>(so + n * OP + 32 * i + 8 * u + 4 * h) = x;
+        for (int u = 0; u < 4; ++u)
+          *reinterpret_cast<float4*>(dst + 32 * i + 8 * u) =
+              make_float4(st.acc[i][4 * u], st.acc[i][4 * u + 1], st.acc[i][4 * u + 2], st.acc[i][4 * u + 3]);
+      if (h == 0) *reinterpret_cast<float2*>(p.ws2 + 2 * at) = make_float2(st.m, l);
     }
-  __syncthreads();
-  constexpr int TPR = 8, DP = D / TPR;                                    // threads a row, values a thread
-  const int rr = threadIdx.x / TPR, part = threadIdx.x % TPR, gr = rt * 32 + rr;
-  if (gr >= R) return;
-  float mx = sm[0][rr];
+  } else {
+    // the waves' shares: o_w relative to m_w, joined at the common maximum
+    if (h == 0) { sm[wave][n] = st.m; sl[wave][n] = l; }
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(buf) + wave * 32 * OP;
 #pragma unroll
-  for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sm[w][rr]);
-  float ls = 0.f, o[DP];
+    for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-  for (int e = 0; e < DP; ++e) o[e] = 0.f;
+      for (int u = 0; u < 4; ++u) {
+        f32x4 x;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const float a = sm[w][rr] == -INFINITY && sl[w][rr] == 0.f ? 0.f : __builtin_amdgcn_exp2f((sm[w][rr] - mx) * p.c);
-    ls += a * sl[w][rr];
-    const float* src = reinterpret_cast<float*>(buf) + (w * 32 + rr) * OP + part * DP;
+        for (int e = 0; e < 4; ++e) x[e] = st.acc[i][4 * u + e];
+        *reinterpret_cast<f32x4*>(so + n * OP + 32 * i + 8 * u + 4 * h) = x;
+      }
+    __syncthreads();
+    constexpr int TPR = 64 * NW / 32, DP = D / TPR;                       // threads a row, values a thread
+    const int rr = threadIdx.x / TPR, part = threadIdx.x % TPR, gr = rt * 32 + rr;
+    if (gr >= R) return;
+    float mx = sm[0][rr];
 #pragma unroll
-    for (int e = 0; e < DP; ++e) o[e] += a == 0.f ? 0.f : a * src[e];
-  }
-  const int gi = gr / p.G, gh = hk * p.G + gr % p.G;
-  const long long grow = ((long long)b * p.H + gh) * p.Lq + gi;
-  if (p.nsplit == 1) {
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sm[w][rr]);
+    float ls = 0.f, o[DP];
+#pragma unroll
+    for (int e = 0; e < DP; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float a = join_factor(sm[w][rr], sl[w][rr], mx, p.c);
+      const float* src = reinterpret_cast<float*>(buf) + (w * 32 + rr) * OP + part * DP;
+      if (a != 0.f) {
+        ls += a * sl[w][rr];
+#pragma unroll
+        for (int e = 0; e < DP; ++e) o[e] += a * src[e];
+      }
+    }
+    const int gi = gr / p.G, gh = hk * p.G + gr % p.G;
     const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
     bf16* dst = p.out + b * p.sob + gi * p.sol + gh * p.soh + part * DP;
 #pragma unroll
@@ -375,44 +398,63 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_split_kernel(AttnP 
       for (int k = 0; k < 4; ++k) x[k] = to16<F16>(o[e + k] * inv);
       *reinterpret_cast<bf16x4*>(dst + e) = x;
     }
-    if (part == 0) p.lse[grow] = ls == 0.f ? -INFINITY : mx * p.scale + __logf(ls);
-  } else {
-    const long long rows = (long long)p.B * p.H * p.Lq;
-    float* dst = p.ws + ((long long)sp * rows + grow) * D + part * DP;
-#pragma unroll
-    for (int e = 0; e < DP; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-    if (part == 0) *reinterpret_cast<float2*>(p.ws2 + 2 * ((long long)sp * rows + grow)) = make_float2(mx, ls);
+    if (part == 0) p.lse[((long long)b * p.H + gh) * p.Lq + gi] = ls == 0.f ? -INFINITY : mx * p.scale + __logf(ls);
   }
 }
 
-// A row's partials of all splits: D / 4 threads a row
+// A row a workgroup: D / 4 threads a split, the splits in turn over the groups of threads, the groups joined in LDS
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnP p) {
-  constexpr int TPR = D / 4;
-  const long long rows = (long long)p.B * p.H * p.Lq;
-  const long long grow = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  const int part = threadIdx.x % TPR;
-  if (threadIdx.x >= 256 / TPR * TPR || grow >= rows) return;
+  constexpr int TPR = D / 4, GR = 256 / TPR;
+  __shared__ float sa[256];
+  __shared__ f32x4 so[GR][TPR];
+  __shared__ float sl[GR];
+  const long long rows = (long long)p.B * p.H * p.Lq, row = blockIdx.x;
+  const int g = threadIdx.x / TPR, part = threadIdx.x % TPR;
+  // the common maximum, then each split's factor, 256 splits at a time
   float mx = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) mx = fmaxf(mx, p.ws2[2 * (s * rows + grow)]);
+  for (int s = threadIdx.x; s < p.nsplit; s += 256) mx = fmaxf(mx, p.ws2[2 * (s * rows + row)]);
+  mx = wave_max(mx);
+  if ((threadIdx.x & 63) == 0) sa[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(sa[0], sa[1]), fmaxf(sa[2], sa[3]));
   float ls = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.ws2 + 2 * (s * rows + grow));
-    const float4 x = *reinterpret_cast<const float4*>(p.ws + (s * rows + grow) * D + 4 * part);
-    const float a = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f((ml.x - mx) * p.c);
-    if (a != 0.f || ml.y != ml.y) {
-      ls += a * ml.y;
-      o.x += a * x.x; o.y += a * x.y; o.z += a * x.z; o.w += a * x.w;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; c0 < p.nsplit; c0 += 256) {
+    const int n = min(256, p.nsplit - c0);
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.ws2 + 2 * ((c0 + threadIdx.x) * rows + row));
+      const float a = join_factor(ml.x, ml.y, mx, p.c);
+      sa[threadIdx.x] = a;
+      if (a != 0.f) ls += a * ml.y;
+    }
+    __syncthreads();
+    if (g < GR) {
+#pragma unroll 8
+      for (int s = g; s < n; s += GR) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p.ws + ((c0 + s) * rows + row) * D + 4 * part);
+        const float a = sa[s];
+        if (a != 0.f) o += a * x;
+      }
     }
   }
+  ls = wave_sum(ls);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sl[threadIdx.x >> 6] = ls;
+  if (g < GR) so[g][part] = o;
+  __syncthreads();
+  if (threadIdx.x >= TPR) return;
+  ls = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  for (int k = 1; k < GR; ++k) o += so[k][part];
   const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
-  const int qi = grow % p.Lq, hq = (grow / p.Lq) % p.H;
-  const long long b = grow / p.Lq / p.H;
+  const int qi = row % p.Lq, hq = (row / p.Lq) % p.H;
+  const long long b = row / p.Lq / p.H;
   bf16x4 y;
-  y[0] = to16<F16>(o.x * inv); y[1] = to16<F16>(o.y * inv); y[2] = to16<F16>(o.z * inv); y[3] = to16<F16>(o.w * inv);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = to16<F16>(o[e] * inv);
   *reinterpret_cast<bf16x4*>(p.out + b * p.sob + qi * p.sol + hq * p.soh + 4 * part) = y;
-  if (part == 0) p.lse[grow] = ls == 0.f ? -INFINITY : mx * p.scale + __logf(ls);
+  if (part == 0) p.lse[row] = ls == 0.f ? -INFINITY : mx * p.scale + __logf(ls);
 }
 
 }  // namespace
@@ -469,7 +511,7 @@ namespace {
 
 struct FwdPlan {
   bool split;
-  int waves;                 // of a tile-kernel workgroup
+  int waves;                 // of a workgroup
   int nblk, nsplit, split_tiles;
   int64_t grid, ws;
 };
@@ -482,17 +524,24 @@ FwdPlan fwd_plan(const LrceAttnDesc* d) {
   f.nblk = (d->Lq + 32 * f.waves - 1) / (32 * f.waves);
   f.grid = (int64_t)d->B * d->H * f.nblk;
   f.nsplit = 1;
-  f.split = rows <= 32 || (f.grid < 128 && d->Lk >= 1024);
+  const int nt = (d->Lk + 31) / 32;
+  const int64_t tiles = (int64_t)d->B * d->Hk * ((rows + 31) / 32);
+  f.split = rows <= 32 || attn_few_rows(tiles, d->Lk);
   if (f.split) {
     f.nblk = (int)((rows + 31) / 32);
-    const int nt = (d->Lk + 31) / 32;
-    const int64_t base = std::max<int64_t>(1, (int64_t)d->B * d->Hk * f.nblk);
-    const int64_t want = (1024 + base - 1) / base;
-    int n = (int)std::max<int64_t>(1, std::min<int64_t>(want, nt / 8));
-    f.split_tiles = std::max(2, ((nt + n - 1) / n + 1) / 2 * 2);
-    f.nsplit = std::max(1, (nt + f.split_tiles - 1) / f.split_tiles);
+    const int64_t base = std::max<int64_t>(1, tiles);
+    f.waves = attn_share_waves(d->D, base);
+    f.split_tiles = std::max(2, (nt + 1) / 2 * 2);
+    if (nt > 32 && base < 512) {
+      // one-wave shares of at least 16 tiles, about two and a half times as many as are resident (LDS: two stages of K and V)
+      const int64_t resident = 256 * std::min<int64_t>(8, 160 * 1024 / (256 * d->D + 512));
+      const int n = (int)std::max<int64_t>(1, std::min<int64_t>((5 * resident / 2 + base - 1) / base, nt / 16));
+      f.waves = 1;
+      f.split_tiles = ((nt + n - 1) / n + 1) / 2 * 2;
+      f.nsplit = (nt + f.split_tiles - 1) / f.split_tiles;
+      f.ws = (int64_t)f.nsplit * d->B * d->H * d->Lq * (d->D + 2);
+    }
     f.grid = base * f.nsplit;
-    if (f.nsplit > 1) f.ws = (int64_t)f.nsplit * d->B * d->H * d->Lq * (d->D + 2);
   }
   return f;
 }
@@ -500,10 +549,13 @@ FwdPlan fwd_plan(const LrceAttnDesc* d) {
 template <int D, bool F16>
 void fwd_launch(const AttnP& p, const FwdPlan& f, hipStream_t s) {
   if (f.split) {
-    attn_split_kernel<D, F16><<<(unsigned)f.grid, 256, 0, s>>>(p);
-    if (f.nsplit > 1) {
-      const int64_t rows = (int64_t)p.B * p.H * p.Lq, per = 256 / (D / 4);
-      attn_join_kernel<D, F16><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(p);
+    if (f.waves == 4) {
+      attn_split_kernel<D, F16, 4><<<(unsigned)f.grid, 256, 0, s>>>(p);
+    } else if (f.waves == 2) {
+      attn_split_kernel<D, F16, 2><<<(unsigned)f.grid, 128, 0, s>>>(p);
+    } else {
+      attn_split_kernel<D, F16, 1><<<(unsigned)f.grid, 64, 0, s>>>(p);
+      attn_join_kernel<D, F16><<<(unsigned)((int64_t)p.B * p.H * p.Lq), 256, 0, s>>>(p);
     }
   } else if (f.waves == 2) {
     if (p.mask) attn_fwd_kernel<D, F16, 2, true><<<(unsigned)f.grid, 128, 0, s>>>(p);

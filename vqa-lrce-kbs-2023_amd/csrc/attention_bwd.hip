@@ -14,6 +14,64 @@
 
 namespace {
 
+// A wave's 32 query rows
+template <int D, bool F16>
+struct DqRow {
+  bf16x8 q[D / 16], g[D / 16];
+  float delta, lse2;
+  __device__ __forceinline__ void init(const AttnP& p, int b, int hq, int bh, int i0, int row, bool valid, int lane, int h, bool tell) {
+    const bf16* qr = p.q + b * p.sqb + row * p.sql + hq * p.sqh;
+    const bf16* gr = p.dout + b * p.sgb + row * p.sgl + hq * p.sgh;
+    const bf16* orow = p.out + b * p.sob + row * p.sol + hq * p.soh;
+    bf16x8 o[D / 16];
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      q[kk] = *reinterpret_cast<const bf16x8*>(qr + 16 * kk + 8 * h);
+      g[kk] = *reinterpret_cast<const bf16x8*>(gr + 16 * kk + 8 * h);
+      o[kk] = *reinterpret_cast<const bf16x8*>(orow + 16 * kk + 8 * h);
+    }
+    const float lse = p.lse[(long long)bh * p.Lq + row];
+    delta = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(from16<F16>(g[kk][j]), from16<F16>(o[kk][j]), delta);
+    attn_landed(q);
+    attn_landed(g);
+    delta += other_half(delta);
+    // a row that sees no key has lse = -inf and p = exp(s - inf) = 0; so have the rows behind the last
+    lse2 = !valid || lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E;
+    const int nst = (p.Lq + 63) / 64 * 2;                                // 32-row blocks of statistics
+    if (tell && i0 / 32 < nst) p.ws[((long long)bh * nst + i0 / 32) * 64 + lane] = h ? (valid ? delta : 0.f) : lse2;
+    // the block that makes their number even
+    if (tell && i0 / 32 == nst - 2 && i0 + 32 >= p.Lq) p.ws[((long long)bh * nst + nst - 1) * 64 + lane] = h ? 0.f : INFINITY;
+  }
+  // the 32 keys from row r0 of the tiles on: bit of ws = key there and not hidden, ls = the last key of the block that the
+  // wave's first row sees
+  __device__ __forceinline__ void block(const AttnP& p, const TileRead<D>& rd, lds_cptr kt, lds_cptr vt, int r0, uint32_t ws, int ls, int n,
+                                        int h, f32x16 (&acc)[D / 32]) const {
+    f32x16 s = mfma32x32x16<F16>(rd.row(kt, r0, 0), q[0], f32x16{}), dp = mfma32x32x16<F16>(rd.row(vt, r0, 0), g[0], f32x16{});
+#pragma unroll
+    for (int kk = 1; kk < D / 16; ++kk) s = mfma32x32x16<F16>(rd.row(kt, r0, kk), q[kk], s);
+#pragma unroll
+    for (int kk = 1; kk < D / 16; ++kk) dp = mfma32x32x16<F16>(rd.row(vt, r0, kk), g[kk], dp);
+    const bool diag = p.causal && ls < 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -lse2)) * (dp[r] - delta);
+    if (diag || ws != ~0u) {
+      const uint32_t kw = (ws & (diag ? upto(ls + n) : ~0u)) >> (4 * h);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = (kw >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : 0.f;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const bf16x8 f = attn_pack<F16>(s, half);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] = mfma32x32x16<F16>(rd.col(kt, r0 + 16 * half, i), f, acc[i]);
+    }
+  }
+};
+
 template <int D, bool F16, int NW>
 __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
   constexpr int KT = 64, TB = KT * D * 2;
@@ -30,29 +88,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
   const int nk = p.causal ? max(0, min(p.Lk, last + p.off + 1)) : p.Lk;
   const int nt = (nk + KT - 1) / KT;
 
-  bf16x8 q[D / 16], g[D / 16];
-  float delta = 0.f;
-  {
-    const bf16* qr = p.q + b * p.sqb + row * p.sql + hq * p.sqh;
-    const bf16* gr = p.dout + b * p.sgb + row * p.sgl + hq * p.sgh;
-    const bf16* orow = p.out + b * p.sob + row * p.sol + hq * p.soh;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      q[kk] = *reinterpret_cast<const bf16x8*>(qr + 16 * kk + 8 * h);
-      g[kk] = *reinterpret_cast<const bf16x8*>(gr + 16 * kk + 8 * h);
-      const bf16x8 o = *reinterpret_cast<const bf16x8*>(orow + 16 * kk + 8 * h);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(from16<F16>(g[kk][j]), from16<F16>(o[j]), delta);
-    }
-  }
-  attn_landed(q);
-  attn_landed(g);
-  delta += other_half(delta);
-  const float lse = p.lse[(long long)bh * p.Lq + row];
-  // a row that sees no key has lse = -inf and p = exp(s - inf) = 0; so have the rows behind the last
-  const float lse2 = !valid || lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E;
-  const int nst = (p.Lq + 63) / 64 * 2;                                  // 32-row blocks of statistics
-  if (i0 / 32 < nst) p.ws[((long long)bh * nst + i0 / 32) * 64 + lane] = h ? (valid ? delta : 0.f) : lse2;
+  DqRow<D, F16> rw;
+  rw.init(p, b, hq, bh, i0, row, valid, lane, h, true);
 
   f32x16 acc[D / 32];
 #pragma unroll
@@ -109,27 +146,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
         const int ls = lim - 32 * sub;                                   // the wave's first row sees keys up to ls of the block
         const uint32_t ws = (uint32_t)(w >> (32 * sub));
         if (ws == 0 || (p.causal && ls + 31 < 0)) continue;
-        f32x16 s, dp;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) s = mfma32x32x16<F16>(rd.row(kt, 32 * sub, kk), q[kk], s);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) dp = mfma32x32x16<F16>(rd.row(vt, 32 * sub, kk), g[kk], dp);
-        const bool diag = p.causal && ls < 31;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -lse2)) * (dp[r] - delta);
-        if (diag || ws != ~0u) {
-          const uint32_t kw = (ws & (diag ? upto(ls + n) : ~0u)) >> (4 * h);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = (kw >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : 0.f;
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const bf16x8 f = attn_pack<F16>(s, half);
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) acc[i] = mfma32x32x16<F16>(rd.col(kt, 32 * sub + 16 * half, i), f, acc[i]);
-        }
+        rw.block(p, rd, kt, vt, 32 * sub, ws, ls, n, h, acc);
       }
       t = tn;
       w = wn;
@@ -139,6 +156,112 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
   bf16* o = p.dq + b * p.dqb + row * p.dql + hq * p.dqh;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) attn_store<F16>(acc[i], p.scale, o + 32 * i, h, valid);
+}
+
+// The same for few rows: the waves of a workgroup have one tile of 32 rows between them, wave w every NW-th key tile of 32,
+// and their sums are added in LDS
+template <int D, bool F16, int NW>
+__global__ void __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) attn_dq_share_kernel(AttnP p) {
+  constexpr int KT = 32, TB = KT * D * 2;
+  typedef TileStage<D, KT, 1> Stage;
+  constexpr int OP = D + 4;
+  constexpr int SZ = NW * 32 * OP * 4 > NW * 4 * TB ? NW * 32 * OP * 4 : NW * 4 * TB;
+  __shared__ __attribute__((aligned(1024))) char buf[SZ];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  const Place at = attn_place(p, p.G);
+  const int blk = p.nblk - 1 - at.blk, b = at.b, hq = at.hq, hk = hq / p.G, bh = b * p.H + hq;
+  const int i0 = blk * 32;
+  const bool valid = i0 + n < p.Lq;
+  const int row = min(i0 + n, p.Lq - 1);
+  const int nk = p.causal ? max(0, min(p.Lk, min(i0 + 31, p.Lq - 1) + p.off + 1)) : p.Lk;
+  const int nt = (nk + KT - 1) / KT;
+  DqRow<D, F16> rw;
+  rw.init(p, b, hq, bh, i0, row, valid, lane, h, wave == 0);
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  TileRead<D> rd;
+  rd.init(lane);
+  Stage sk, sv;
+  sk.init(lane, 0, p.skl);
+  sv.init(lane, 0, p.svl);
+  const char* kb = uni(p.k + b * p.skb + hk * p.skh);
+  const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  const long long kstep = p.skl * (2 * KT), vstep = p.svl * (2 * KT);
+  lds_ptr lds = (lds_ptr)buf + wave * (4 * TB);
+  const int chunk = p.mask ? 128 : max(nt, 1);
+  for (int c0 = 0; c0 < nt; c0 += chunk) {
+    const int c1 = min(nt, c0 + chunk);
+    uint32_t mlo = 0, mhi = 0;
+    if (p.mask)
+      attn_mask_words<1>(p, b, c0 / 2, (c1 + 1) / 2, lane, [&](int w, uint64_t bits) {
+        if (lane == w - c0 / 2) { mlo = (uint32_t)bits; mhi = (uint32_t)(bits >> 32); }
+      });
+    auto next = [&](int t, uint32_t& w) {
+      for (; t < c1; t += NW) {
+        w = p.mask ? (uint32_t)__builtin_amdgcn_readlane(((t - c0) & 1) ? mhi : mlo, (t - c0) >> 1) : (uint32_t)low_bits(p.Lk - t * KT);
+        if (w != 0) break;
+      }
+      return t;
+    };
+    auto stage = [&](int t, uint32_t w, int cur) {
+      const char *ka = kb + t * kstep, *va = vb + t * vstep;
+      const uint32_t kd = attn_lds_u32(lds + 2 * cur * TB), vd = attn_lds_u32(lds + (2 * cur + 1) * TB);
+      const int m = p.Lk - t * KT;
+      if (p.mask && w != ~0u) {
+        sk.load(ka, m, w, kd, lane, 0);
+        sv.load(va, m, w, vd, lane, 0);
+      } else {
+        sk.load(ka, m, kd, 0);
+        sv.load(va, m, vd, 0);
+      }
+    };
+    uint32_t w0 = 0, w1 = 0, w2 = 0;
+    int cur = 0;
+    int t0 = next(wave + c0, w0);
+    if (t0 < c1) stage(t0, w0, 0);
+    int t1 = next(t0 + NW, w1);
+    if (t1 < c1) stage(t1, w1, 1);
+    while (t0 < c1) {
+      if (t1 < c1) attn_wait_vm<2 * Stage::NI>();
+      else attn_wait_vm<0>();
+      rw.block(p, rd, lds + 2 * cur * TB, lds + (2 * cur + 1) * TB, 0, w0, i0 + p.off - t0 * KT, n, h, acc);
+      const int t2 = next(t1 + NW, w2);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the tile's reads are done: its place may be filled
+      if (t2 < c1) stage(t2, w2, cur);
+      t0 = t1; w0 = w1;
+      t1 = t2; w1 = w2;
+      cur ^= 1;
+    }
+  }
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(buf) + wave * 32 * OP;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = acc[i][4 * u + e];
+      *reinterpret_cast<f32x4*>(so + n * OP + 32 * i + 8 * u + 4 * h) = x;
+    }
+  __syncthreads();
+  constexpr int TPR = 64 * NW / 32, DP = D / TPR;
+  const int rr = threadIdx.x / TPR, part = threadIdx.x % TPR;
+  if (i0 + rr >= p.Lq) return;
+  bf16* dst = p.dq + b * p.dqb + (long long)(i0 + rr) * p.dql + hq * p.dqh + part * DP;
+#pragma unroll
+  for (int e = 0; e < DP; e += 4) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) o += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(buf) + (w * 32 + rr) * OP + part * DP + e);
+    bf16x4 x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = to16<F16>(o[k] * p.scale);
+    *reinterpret_cast<bf16x4*>(dst + e) = x;
+  }
 }
 
 // Query tiles of 64 rows (two blocks of 32) of one head at a time; the heads of the group one after the other.  With
@@ -162,20 +285,6 @@ __global__ void __launch_bounds__(NW * 64, D <= 96 ? 2 : 1) attn_dkv_kernel(Attn
   const bool some = __any(keep), allk = __all(keep);
   const bool work = __syncthreads_or(some);
 
-  bf16x8 kf[D / 16], vf[D / 16];
-  {
-    const long long jr = min(j, p.Lk - 1);
-    const bf16* kr = p.k + b * p.skb + jr * p.skl + hk * p.skh;
-    const bf16* vr = p.v + b * p.svb + jr * p.svl + hk * p.svh;
-    const bf16x8 zero = {};
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      kf[kk] = keep ? *reinterpret_cast<const bf16x8*>(kr + 16 * kk + 8 * h) : zero;
-      vf[kk] = keep ? *reinterpret_cast<const bf16x8*>(vr + 16 * kk + 8 * h) : zero;
-    }
-    attn_landed(kf);
-    attn_landed(vf);
-  }
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -209,6 +318,20 @@ __global__ void __launch_bounds__(NW * 64, D <= 96 ? 2 : 1) attn_dkv_kernel(Attn
   };
   int cur = 0, tc = ts;
   if (e0 < e1) stage(0);
+  bf16x8 kf[D / 16], vf[D / 16];
+  {
+    const long long jr = min(j, p.Lk - 1);
+    const bf16* kr = p.k + b * p.skb + jr * p.skl + hk * p.skh;
+    const bf16* vr = p.v + b * p.svb + jr * p.svl + hk * p.svh;
+    const bf16x8 zero = {};
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      kf[kk] = keep ? *reinterpret_cast<const bf16x8*>(kr + 16 * kk + 8 * h) : zero;
+      vf[kk] = keep ? *reinterpret_cast<const bf16x8*>(vr + 16 * kk + 8 * h) : zero;
+    }
+    attn_landed(kf);
+    attn_landed(vf);
+  }
   for (int e = e0; e < e1; ++e) {
     attn_barrier();
     if (e + 1 < e1) stage(cur ^ 1);
@@ -302,6 +425,7 @@ __global__ void __launch_bounds__(256) attn_dkv_sum_kernel(AttnP p) {
 }
 
 struct BwdPlan {
+  bool share;
   int wq, wk, nbq, nbk, nsplit;
   int64_t gq, gk, stat, part;
 };
@@ -310,7 +434,10 @@ BwdPlan bwd_plan(const LrceAttnDesc* d) {
   BwdPlan f{};
   f.wq = d->Lq <= 64 ? 2 : 4;
   f.wk = d->Lk <= 64 ? 2 : 4;
-  f.nbq = (d->Lq + 32 * f.wq - 1) / (32 * f.wq);
+  const int64_t row_tiles = (int64_t)d->B * d->H * ((d->Lq + 31) / 32);
+  f.share = attn_few_rows(row_tiles, d->Lk);
+  if (f.share) f.wq = attn_share_waves(d->D, row_tiles);
+  f.nbq = f.share ? (d->Lq + 31) / 32 : (d->Lq + 32 * f.wq - 1) / (32 * f.wq);
   f.nbk = (d->Lk + 32 * f.wk - 1) / (32 * f.wk);
   f.gq = (int64_t)d->B * d->H * f.nbq;
   f.stat = (int64_t)d->B * d->H * ((d->Lq + 63) / 64) * 128;
@@ -325,7 +452,9 @@ template <int D, bool F16>
 void bwd_launch(AttnP p, const BwdPlan& f, hipStream_t s) {
   if (f.gq) {
     p.nblk = f.nbq;
-    if (f.wq == 2) attn_dq_kernel<D, F16, 2><<<(unsigned)f.gq, 128, 0, s>>>(p);
+    if (f.share && f.wq == 2) attn_dq_share_kernel<D, F16, 2><<<(unsigned)f.gq, 128, 0, s>>>(p);
+    else if (f.share) attn_dq_share_kernel<D, F16, 4><<<(unsigned)f.gq, 256, 0, s>>>(p);
+    else if (f.wq == 2) attn_dq_kernel<D, F16, 2><<<(unsigned)f.gq, 128, 0, s>>>(p);
     else attn_dq_kernel<D, F16, 4><<<(unsigned)f.gq, 256, 0, s>>>(p);
   }
   if (f.gk) {

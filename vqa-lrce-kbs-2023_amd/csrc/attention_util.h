@@ -35,6 +35,14 @@ struct AttnP {
 int attn_check(const LrceAttnDesc* d, const char* what);
 void attn_fill(const LrceAttnDesc* d, AttnP& p);
 
+// Whether the waves of a workgroup share 32 rows and divide the keys, rather than have 32 rows each: where row tiles alone
+// leave the chip's 1024 SIMDs without a second wave to fill the first one's waits, and the key axis is long enough to divide.
+// Measured (64 heads, 1024 keys, d 64, forward): 512 row tiles 10.9 us divided, 21.6 us not; 1024 row tiles 21 us either way.
+inline bool attn_few_rows(int64_t row_tiles, int Lk) { return row_tiles <= 768 && Lk >= 192; }
+// ... and how many waves: a wave has two stages of K and V of 32 keys in LDS (8 to 32 KB); four waves of the wide ones would
+// leave one workgroup a CU
+inline int attn_share_waves(int D, int64_t row_tiles) { return D <= 64 || row_tiles <= 256 ? 4 : 2; }
+
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -201,20 +209,35 @@ struct TileStage {
   }
 };
 
-// Mask bits of the 64-key tiles [t0, t0 + n) of batch row b: bit j of word w = key 64 (t0 + w) + j is there and not hidden
+// Mask bits of the 64-key words w0, w0 + STEP, ... below w1 of batch row b: put(word, bits), bit l = key 64 word + l is there and
+// not hidden.  Up to eight words are loaded before the first is looked at.
+template <int STEP, typename T, typename F>
+__device__ __forceinline__ void attn_mask_words_of(const T* m, int Lk, int w0, int w1, int lane, F&& put) {
+  for (int c = w0; c < w1; c += 8 * STEP) {
+    T x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i * STEP < w1) x[i] = m[min((c + i * STEP) * 64 + lane, Lk - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int w = c + i * STEP;
+      if (w < w1) put(w, __ballot(x[i] != 0 && w * 64 + lane < Lk));
+    }
+  }
+}
+template <int STEP, typename F>
+__device__ __forceinline__ void attn_mask_words(const AttnP& p, int b, int w0, int w1, int lane, F&& put) {
+  const long long at = (long long)b * p.smb;
+  if (p.mask_bytes == 1) attn_mask_words_of<STEP>(static_cast<const uint8_t*>(p.mask) + at, p.Lk, w0, w1, lane, put);
+  else if (p.mask_bytes == 4) attn_mask_words_of<STEP>(static_cast<const int*>(p.mask) + at, p.Lk, w0, w1, lane, put);
+  else attn_mask_words_of<STEP>(static_cast<const long long*>(p.mask) + at, p.Lk, w0, w1, lane, put);
+}
+// ... of the tiles [t0, t0 + n) to LDS
 template <int NW>
 __device__ __forceinline__ void attn_pack_mask(const AttnP& p, int b, int t0, int n, LRCE_LDS uint64_t* words, int lane, int wave) {
-  for (int w = wave; w < n; w += NW) {
-    const int j = (t0 + w) * 64 + lane;
-    bool on = j < p.Lk;
-    if (on) {
-      const long long at = (long long)b * p.smb + j;
-      on = p.mask_bytes == 1 ? static_cast<const uint8_t*>(p.mask)[at] != 0
-         : p.mask_bytes == 4 ? static_cast<const int*>(p.mask)[at] != 0 : static_cast<const long long*>(p.mask)[at] != 0;
-    }
-    const uint64_t bits = __ballot(on);
-    if (lane == 0) words[w] = bits;
-  }
+  attn_mask_words<NW>(p, b, t0 + wave, t0 + n, lane, [&](int w, uint64_t bits) {
+    if (lane == 0) words[w - t0] = bits;
+  });
 }
 __device__ __forceinline__ uint64_t uni64(uint64_t x) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x) |
