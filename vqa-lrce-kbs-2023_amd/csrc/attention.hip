@@ -195,6 +195,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_fwd_kernel(AttnP p) {
       lds_cptr kt = lds + (cur ^ 1) * TB, vt = lds + (2 + cur) * TB;
       f32x16 sn[2];
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);                                     // the wave with matrix work first: 3 - 7 % at 2 waves a SIMD
       sn[0] = st.scores(rd, kt, 0);
       st.weigh(s[0], p0, p.c, mc);
       attn_interleave<D / 16, 128 / D * 7>();
@@ -205,6 +206,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_fwd_kernel(AttnP p) {
       attn_interleave<D / 8, 128 / D * 4>();
       __builtin_amdgcn_sched_barrier(0);
       st.sum(rd, vt, 32, p1);
+      __builtin_amdgcn_s_setprio(0);
       mask(t1, w1, sn);
       mx = st.template top<2>(sn);
       s[0] = sn[0];

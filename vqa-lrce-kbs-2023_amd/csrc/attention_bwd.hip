@@ -46,29 +46,58 @@ struct DqRow {
     // the block that makes their number even
     if (tell && i0 / 32 == nst - 2 && i0 + 32 >= p.Lq) p.ws[((long long)bh * nst + nst - 1) * 64 + lane] = h ? 0.f : INFINITY;
   }
-  // the 32 keys from row r0 of the tiles on: bit of ws = key there and not hidden, ls = the last key of the block that the
-  // wave's first row sees
-  __device__ __forceinline__ void block(const AttnP& p, const TileRead<D>& rd, lds_cptr kt, lds_cptr vt, int r0, uint32_t ws, int ls, int n,
-                                        int h, f32x16 (&acc)[D / 32]) const {
-    f32x16 s = mfma32x32x16<F16>(rd.row(kt, r0, 0), q[0], f32x16{}), dp = mfma32x32x16<F16>(rd.row(vt, r0, 0), g[0], f32x16{});
+  // the 32 keys from row r0 of the tiles on: weights and dout . v (bit of ws = key there and not hidden, ls = the last key of the
+  // block that the wave's first row sees; hidden pairs have weight 0)
+  __device__ __forceinline__ void pairs(const AttnP& p, const TileRead<D>& rd, lds_cptr kt, lds_cptr vt, int r0, uint32_t ws, int ls, int n,
+                                        int h, f32x16& s, f32x16& dp) const {
+    s = mfma32x32x16<F16>(rd.row(kt, r0, 0), q[0], f32x16{});
+    dp = mfma32x32x16<F16>(rd.row(vt, r0, 0), g[0], f32x16{});
 #pragma unroll
     for (int kk = 1; kk < D / 16; ++kk) s = mfma32x32x16<F16>(rd.row(kt, r0, kk), q[kk], s);
 #pragma unroll
     for (int kk = 1; kk < D / 16; ++kk) dp = mfma32x32x16<F16>(rd.row(vt, r0, kk), g[kk], dp);
-    const bool diag = p.causal && ls < 31;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -lse2)) * (dp[r] - delta);
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -lse2));
+    const bool diag = p.causal && ls < 31;
     if (diag || ws != ~0u) {
       const uint32_t kw = (ws & (diag ? upto(ls + n) : ~0u)) >> (4 * h);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = (kw >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : 0.f;
     }
+  }
+  __device__ __forceinline__ void sum(const TileRead<D>& rd, lds_cptr kt, int r0, f32x16& s, const f32x16& dp, f32x16 (&acc)[D / 32]) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const bf16x8 f = attn_pack<F16>(s, half);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) acc[i] = mfma32x32x16<F16>(rd.col(kt, r0 + 16 * half, i), f, acc[i]);
     }
+  }
+  __device__ __forceinline__ void block(const AttnP& p, const TileRead<D>& rd, lds_cptr kt, lds_cptr vt, int r0, uint32_t ws, int ls, int n,
+                                        int h, f32x16 (&acc)[D / 32]) const {
+    f32x16 s, dp;
+    pairs(p, rd, kt, vt, r0, ws, ls, n, h, s, dp);
+    sum(rd, kt, r0, s, dp, acc);
+  }
+  // All that the rows see, in at most two blocks (at kt, vt and kt + step, vt + step): delta is the sum of weight times dout . v,
+  // from a first walk over them.  The one from out would carry out's rounding to 16 bits, which counts where a few weights
+  // are large (it falls off as 1 / keys).
+  __device__ __forceinline__ void few(const AttnP& p, const TileRead<D>& rd, lds_cptr kt, lds_cptr vt, int step, uint32_t w0, int l0, uint32_t w1,
+                                      int l1, int bh, int i0, bool valid, int lane, int h) {
+    float d = 0.f;
+#pragma unroll 1
+    for (int x = 0; x < 2; ++x) {
+      const uint32_t w = x ? w1 : w0;
+      if (w == 0) continue;
+      f32x16 s, dp;
+      pairs(p, rd, kt + x * step, vt + x * step, 0, w, x ? l1 : l0, lane & 31, h, s, dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) d = __builtin_fmaf(s[r], dp[r], d);
+    }
+    delta = d + other_half(d);
+    if (h && valid) p.ws[((long long)bh * ((p.Lq + 63) / 64 * 2) + i0 / 32) * 64 + lane] = delta;
   }
 };
 
@@ -87,6 +116,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
   const int last = min(blk * (32 * NW) + 32 * NW, p.Lq) - 1;
   const int nk = p.causal ? max(0, min(p.Lk, last + p.off + 1)) : p.Lk;
   const int nt = (nk + KT - 1) / KT;
+  const int tw = p.causal ? min(nt, max(0, i0 + 31 + p.off + KT) / KT) : nt;   // tiles from tw on hold no key that this wave's rows see
 
   DqRow<D, F16> rw;
   rw.init(p, b, hq, bh, i0, row, valid, lane, h, true);
@@ -134,6 +164,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
     };
     uint64_t w = 0, wn = 0;
     int t = next(c0, w), cur = 0;
+    const int t_end = min(c1, tw);
+    bool only = c0 == 0 && (c1 == nt || tw <= c1);                       // (until a second tile is found) the rows' keys lie in one tile
     if (t < c1) stage(t, w, 0);
     while (t < c1) {
       attn_barrier();
@@ -141,6 +173,9 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_dq_kernel(AttnP p) {
       if (tn < c1) stage(tn, wn, cur ^ 1);
       const int lim = i0 + p.off - t * KT;
       lds_cptr kt = lds + 2 * cur * TB, vt = lds + (2 * cur + 1) * TB;
+      only = only && tn >= t_end;
+      if (only && t < t_end)
+        rw.few(p, rd, kt, vt, TB / 2, (uint32_t)w, lim, p.causal && lim < 1 ? 0u : (uint32_t)(w >> 32), lim - 32, bh, i0, valid, lane, h);
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
         const int ls = lim - 32 * sub;                                   // the wave's first row sees keys up to ls of the block
@@ -199,8 +234,12 @@ __global__ void __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) attn_dq_share_kernel
       attn_mask_words<1>(p, b, c0 / 2, (c1 + 1) / 2, lane, [&](int w, uint64_t bits) {
         if (lane == w - c0 / 2) { mlo = (uint32_t)bits; mhi = (uint32_t)(bits >> 32); }
       });
+    // few visible tiles: the first wave has them all
+    const int seen = p.mask ? __popcll(__ballot(mlo != 0)) + __popcll(__ballot(mhi != 0)) : nt;
+    const bool few = nt <= chunk && seen <= 2;
+    const int step = few ? 1 : NW;
     auto next = [&](int t, uint32_t& w) {
-      for (; t < c1; t += NW) {
+      for (; t < c1; t += step) {
         w = p.mask ? (uint32_t)__builtin_amdgcn_readlane(((t - c0) & 1) ? mhi : mlo, (t - c0) >> 1) : (uint32_t)low_bits(p.Lk - t * KT);
         if (w != 0) break;
       }
@@ -220,15 +259,19 @@ __global__ void __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) attn_dq_share_kernel
     };
     uint32_t w0 = 0, w1 = 0, w2 = 0;
     int cur = 0;
-    int t0 = next(wave + c0, w0);
+    int t0 = few && wave ? c1 : next(wave + c0, w0);
     if (t0 < c1) stage(t0, w0, 0);
-    int t1 = next(t0 + NW, w1);
+    int t1 = next(t0 + step, w1);
     if (t1 < c1) stage(t1, w1, 1);
+    if (few && t0 < c1) {
+      attn_wait_vm<0>();
+      rw.few(p, rd, lds, lds + TB, 2 * TB, w0, i0 + p.off - t0 * KT, t1 < c1 ? w1 : 0u, i0 + p.off - t1 * KT, bh, i0, valid, lane, h);
+    }
     while (t0 < c1) {
       if (t1 < c1) attn_wait_vm<2 * Stage::NI>();
       else attn_wait_vm<0>();
       rw.block(p, rd, lds + 2 * cur * TB, lds + (2 * cur + 1) * TB, 0, w0, i0 + p.off - t0 * KT, n, h, acc);
-      const int t2 = next(t1 + NW, w2);
+      const int t2 = next(t1 + step, w2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the tile's reads are done: its place may be filled
       if (t2 < c1) stage(t2, w2, cur);
       t0 = t1; w0 = w1;
