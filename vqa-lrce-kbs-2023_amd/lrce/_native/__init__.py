@@ -316,12 +316,16 @@ def stream_of(t):
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+_profiling = torch._C._autograd._profiler_enabled
+
+
 def call(name, *args):
-    if torch._C._autograd._profiler_enabled():
+    fn = getattr(_lib or lib(), name)
+    if _profiling():
         # visible in torch.profiler traces as lrce::<entry point> (the launch itself is async)
         with torch.profiler.record_function("lrce::" + name[5:]):
-            rc = getattr(lib(), name)(*args)
+            rc = fn(*args)
     else:
-        rc = getattr(lib(), name)(*args)
+        rc = fn(*args)
     if rc != 0:
         raise NativeError(f"{name} failed ({rc}): {lib().lrce_last_error().decode()}")

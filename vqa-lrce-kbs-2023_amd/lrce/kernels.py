@@ -665,12 +665,13 @@ _TYPE = {BF16: 0, F16: 1, F32: 2}
 _ATTN_PACK = struct.Struct("6P13q9ifPq4P12q").pack
 _ROPE_PACK = struct.Struct("13Pq18qq9if").pack
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _call_on(name, t, *args):
     """N.call on t's current stream, with t's device as the current one: a launch goes to the device of its stream."""
     dev = t.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         return call(name, *args, _raw_stream(dev))
     with torch.cuda.device(dev):
         return call(name, *args, _raw_stream(dev))
@@ -691,6 +692,9 @@ def _head_rows(t):
 
 def _head_rows16(t):
     """_head_rows of t, or of a copy where its rows are not the whole 16-byte pieces that the kernels read."""
+    if t.is_contiguous() and not t.data_ptr() & 15:       # (the head dim is a multiple of 32)
+        _, n, h, d = t.shape
+        return t, n * h * d, h * d, d
     r = _head_rows(t)
     if (r[1] | r[2] | r[3]) & 7 or r[2] >= 1 << 23 or r[0].data_ptr() & 15:
         return _head_rows(t.clone(memory_format=torch.contiguous_format))
