@@ -125,7 +125,7 @@ struct Pairs {
 
 // NCH chunks of VEC pairs a lane (2 only where VEC = 1 and D > 128)
 template <typename T, int VEC, int NCH, bool BWD>
-__global__ void __launch_bounds__(256, BWD ? 3 : 5) qk_rope_kernel(RopeP p) {
+__global__ void __launch_bounds__(256, BWD ? (VEC == 8 ? 3 : 4) : 5) qk_rope_kernel(RopeP p) {
   constexpr int W = 2 * VEC;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lanes = 1 << p.lgrp, ngrp = 64 >> p.lgrp, grp = lane >> p.lgrp, li = lane & (lanes - 1);
@@ -295,8 +295,8 @@ int rope_check(const LrceRopeDesc* d, bool bwd, const char* what) {
   return LRCE_OK;
 }
 
-// The backward leaves a row of partial sums a workgroup, four waves of at least a token each: up to the 3 workgroups a CU that are resident
-int64_t rope_wgs(int64_t tokens) { return std::max<int64_t>(1, std::min<int64_t>((tokens + 3) / 4, 768)); }
+// The backward leaves a row of partial sums a workgroup, four waves of at least a token each: up to 4 workgroups a CU
+int64_t rope_wgs(int64_t tokens) { return std::max<int64_t>(1, std::min<int64_t>((tokens + 3) / 4, 1024)); }
 
 struct RopePlan { int vec, lgrp, gpt, tpw; };
 
@@ -385,7 +385,7 @@ extern "C" int lrce_qk_norm_rope_bwd(const LrceRopeDesc* d, void* stream) {
   const RopePlan f = rope_plan(d, true);
   RopeP p;
   rope_fill(d, f, p);
-  p.nwg = (int)rope_wgs(p.tokens);
+  p.nwg = (int)std::min<int64_t>(rope_wgs(p.tokens), f.vec == 8 ? 768 : 1024);   // what is resident: 3 or 4 waves a SIMD (1024 of 768: 268 us, not 207)
   if (!d->workspace || d->workspace_elems < (int64_t)p.nwg * 2 * d->D)
     return lrce_fail(LRCE_E_ARG, "qk_norm_rope_bwd: a workspace of %lld floats is needed", (long long)p.nwg * 2 * d->D);
   hipStream_t s = static_cast<hipStream_t>(stream);

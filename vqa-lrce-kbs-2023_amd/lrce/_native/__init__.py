@@ -33,6 +33,23 @@ def lib():
     return _lib
 
 
+_bound = None
+
+
+def binding():
+    """The module built from csrc/binding.cpp, bound to the library's entry points."""
+    global _bound
+    if _bound is None:
+        L = lib()
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise NativeError(f"_binding.so not built or not loadable ({e}); run `python __graft_entry__.py` / make -C csrc") from e
+        _binding.bind(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND))
+        _bound = _binding
+    return _bound
+
+
 def loaded():
     return _lib is not None
 
@@ -291,6 +308,12 @@ _RET.update({"lrce_dec_step_field": _I64, "lrce_dec_step_ws_elems": _I64, "lrce_
 _SIGS["lrce_layernorm_bwd_workspace"] = [_I, _I]
 _RET.update({n: _I64 for n in ("lrce_attn_fwd_workspace", "lrce_attn_bwd_workspace", "lrce_qk_norm_rope_bwd_workspace",
                                "lrce_embedding_bwd_workspace")})
+
+
+# the entry points that _binding calls, in bind()'s order
+_BOUND = ("lrce_attn_fwd", "lrce_attn_bwd", "lrce_attn_fwd_workspace", "lrce_attn_bwd_workspace", "lrce_qk_norm_rope_fwd",
+          "lrce_qk_norm_rope_bwd", "lrce_qk_norm_rope_bwd_workspace", "lrce_embedding_fwd", "lrce_embedding_bwd",
+          "lrce_embedding_bwd_workspace")
 
 
 def _declare(L):

@@ -666,6 +666,16 @@ _ATTN_PACK = struct.Struct("6P13q9ifPq4P12q").pack
 _ROPE_PACK = struct.Struct("13Pq18qq9if").pack
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_profiling = torch._C._autograd._profiler_enabled
+
+
+def _direct(t):
+    """(binding, current device, its stream) where t may take the interpreter-free host path (csrc/binding.cpp): t on a device,
+    no profiler that the call should appear in.  The binding answers None for all but the plain case."""
+    if not t.is_cuda or _profiling():
+        return None, 0, 0
+    dev = _current_device()
+    return N.binding(), dev, _raw_stream(dev)
 
 
 def _call_on(name, t, *args):
@@ -751,6 +761,9 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
     key_mask [B, Lk] (bool or integer, 0 = hidden); causal: row i sees the keys j <= i + Lk - Lq; scale (positive): D ** -0.5 by
     default.  A row that sees no key gives 0 and lse -inf.  k and v may hold anything at keys that key_mask hides; at keys
     that only causality hides they must be finite.  lse is the natural logarithm of the row's sum, for attention_bwd."""
+    b, dev, stream = _direct(q)
+    if b and (r := b.attention(q, k, v, key_mask, causal, scale, dev, stream)):
+        return r
     B, Lq, H, D, Lk, Hk, m, scale = _attn_args("attention", q, k, v, key_mask, scale)
     q, *qs = _head_rows16(q)
     k, *ks = _head_rows16(k)
@@ -769,6 +782,9 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
 def attention_bwd(dout, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
     """(dq, dk, dv) of attention() for dout, with the forward's out and lse; the arguments as there.  Sums over the query
     heads that share a key head are formed in f32; the result does not depend on timing."""
+    b, dev, stream = _direct(q)
+    if b and (r := b.attention_bwd(q, k, v, key_mask, causal, scale, dout, out, lse, dev, stream)):
+        return r
     B, Lq, H, D, Lk, Hk, m, scale = _attn_args("attention_bwd", q, k, v, key_mask, scale)
     dev, shape = q.get_device(), q.shape
     if not (dout.dtype is q.dtype and out.dtype is q.dtype and dout.shape == shape and out.shape == shape and dout.get_device() == dev
@@ -831,6 +847,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
     multiple of 8 up to 256) divided by its root mean square (eps inside the root), times its weight (f32 [D]), then its first
     R = 2 len(inv_freq) dims rotated by positions * inv_freq: pairs (i, R/2 + i), or (2i, 2i + 1) with interleaved.
     positions int32 / int64 [B, L] or [L]; inv_freq f32; the angles are formed in 64 bits, all else in f32 with one rounding."""
+    b, dev, stream = _direct(q)
+    if b and (r := b.qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, dev, stream)):
+        return r
     B, L, H, Hk, D = _rope_args("qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, eps)
     q, *qs = _head_rows(q)
     k, *ks = _head_rows(k)
@@ -848,6 +867,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
 def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """(dq, dk, dq_weight, dk_weight) of qk_norm_rope() for the gradients of its outputs; the other arguments as there.  The
     weights' gradients (f32) are summed in a fixed order."""
+    b, dev, stream = _direct(q)
+    if b and (r := b.qk_norm_rope_bwd(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, dq_out, dk_out, dev, stream)):
+        return r
     B, L, H, Hk, D = _rope_args("qk_norm_rope_bwd", q, k, q_weight, k_weight, positions, inv_freq, eps)
     if not (dq_out.dtype is q.dtype and dk_out.dtype is q.dtype and dq_out.shape == q.shape and dk_out.shape == k.shape
             and dq_out.get_device() == dk_out.get_device() == q.get_device()):
@@ -888,6 +910,9 @@ def _embed_ids(what, ids, dev):
 def embedding(ids, weight, scale=1.0, out_dtype=None):
     """scale * weight[ids]: ids (any shape) int32 / int64, weight [rows, cols] bf16, fp16 or f32 (rows may be strided); the result
     has weight's type, or out_dtype where weight is f32.  An id outside the table gives a row of NaN (no host check)."""
+    b, dev, stream = _direct(weight)
+    if b and (r := b.embedding(ids, weight, scale, out_dtype, dev, stream)) is not None:
+        return r
     out_dtype = weight.dtype if out_dtype is None else out_dtype
     if not (weight.is_cuda and weight.dim() == 2 and weight.dtype in _TYPE and out_dtype in _TYPE
             and (weight.dtype is F32 or out_dtype is weight.dtype) and weight.shape[0] > 0 and weight.shape[1] > 0):
@@ -916,6 +941,9 @@ def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=-1, dw=None):
     """The gradient of embedding()'s table for dy [*ids.shape, cols] (bf16, fp16 or f32): f32 [rows, cols], row v = scale * the sum
     of dy over the places where ids is v, in their order (the same bits each time); padding_idx (-1: none) and ids outside the
     table have none.  dw: a contiguous f32 [rows, cols] the gradient is added to (and returned) instead of a new tensor."""
+    b, dev, stream = _direct(dy) if dw is None else (None, 0, 0)
+    if b and (r := b.embedding_bwd(dy, ids, rows, scale, padding_idx, dev, stream)) is not None:
+        return r
     if not (dy.is_cuda and dy.dtype in _TYPE):
         _chk(dy, None, "embedding_bwd: dy")
         raise N.NativeError(f"embedding_bwd: dy must be bf16, fp16 or f32, got {dy.dtype}")
