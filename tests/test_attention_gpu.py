@@ -75,3 +75,37 @@ def test_single_tokens_over_a_long_axis(D):
     for B, Lq, Lk, H, Hk, causal, mask in ((1, 1, 20000, 8, 1, False, None), (3, 1, 9001, 10, 2, False, "random"), (2, 5, 3000, 8, 2, True, "tail"),
                                            (2, 1, 200, 4, 4, False, "blocks"), (1, 40, 4096, 2, 1, True, None), (40, 1, 1000, 24, 8, True, "tail")):
         run(*make(B, Lq, Lk, H, Hk, D, "bf16", seed=Lk, mask=mask), causal=causal, backward=False, what=f"{B} {Lq} {Lk} {H} {Hk}")
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_rows_over_many_keys(D, dtype):
+    """Enough row tiles that a workgroup's waves take rows of their own, over several key tiles."""
+    for Lq, Lk, causal, mask in ((401, 500, False, None), (401, 500, True, "tail"), (500, 401, True, None), (416, 321, False, "blocks"),
+                                 (385, 192, True, "random")):
+        run(*make(3, Lq, Lk, 24, 6, D, dtype, seed=Lq, mask=mask), causal=causal, what=f"{Lq} {Lk} {causal} {mask}")
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_middling_rows_over_many_keys(D):
+    """256 to 768 row tiles: the waves of a workgroup divide the keys."""
+    for B, Lq, Lk, H, Hk, causal, mask in ((4, 257, 613, 8, 8, False, None), (5, 250, 700, 12, 4, True, "tail"), (4, 333, 449, 10, 5, False, "random"),
+                                           (6, 200, 192, 8, 2, True, "blocks")):
+        run(*make(B, Lq, Lk, H, Hk, D, "bf16", seed=Lq, mask=mask), causal=causal, what=f"{B} {Lq} {Lk} {H} {Hk}")
+
+
+@pytest.mark.parametrize("D", [64, 96])
+def test_masks_longer_than_a_workgroup_reads_at_once(D):
+    """The mask's words are read 4096 keys (keys divided over the waves) or 16384 keys (rows divided) at a time."""
+    run(*make(64, 1, 4500, 8, 8, D, "bf16", seed=1, mask="tail"), what="a workgroup for each cache")
+    run(*make(70, 3, 4200, 8, 8, D, "bf16", seed=2, mask="random"), causal=True, what="a workgroup for each cache, causal")
+
+
+@pytest.mark.parametrize("mask,causal", [("random", False), ("tail", True)])
+def test_masks_longer_than_16384_keys(mask, causal):
+    run(*make(2, 820, 16500, 16, 2, 32, "bf16", seed=3, mask=mask), causal=causal)
+
+
+def test_backward_of_single_tokens_over_long_caches():
+    for B, Lq, Lk, H, Hk, D, causal, mask in ((2, 1, 9001, 8, 2, 128, False, "tail"), (1, 1, 20000, 4, 4, 64, True, None), (3, 2, 5000, 12, 3, 96, True, "random")):
+        run(*make(B, Lq, Lk, H, Hk, D, "bf16", seed=Lk, mask=mask), causal=causal, what=f"{B} {Lq} {Lk} {H} {Hk}")

@@ -175,3 +175,9 @@ def test_embedding_ids_outside_the_table_and_shapes():
     assert torch.equal(K().embedding_bwd(torch.zeros(0, 16, device=dev), none, 10), torch.zeros(10, 16, device=dev))
     wide = torch.randn(10, 40, device=dev)[:, 5:21]           # rows of a wider table, not aligned
     assert torch.equal(K().embedding(ids[1:, :2], wide), wide[ids[1:, :2]])
+
+
+@pytest.mark.parametrize("N,V,C", [(300001, 1000, 8), (270000, (1 << 18) + 5, 5), (9000, 600000, 3), (5000, 1 << 19, 16), (100, 1 << 21, 2)])
+def test_embedding_of_many_tokens_and_wide_tables(N, V, C):
+    """More than 2^18 tokens (more places a workgroup), ids of 19 and 20 bits (three passes of the sort)."""
+    test_embedding(N, V, C, ("f32", "f32", "f32"))
