@@ -109,3 +109,12 @@ def test_masks_longer_than_16384_keys(mask, causal):
 def test_backward_of_single_tokens_over_long_caches():
     for B, Lq, Lk, H, Hk, D, causal, mask in ((2, 1, 9001, 8, 2, 128, False, "tail"), (1, 1, 20000, 4, 4, 64, True, None), (3, 2, 5000, 12, 3, 96, True, "random")):
         run(*make(B, Lq, Lk, H, Hk, D, "bf16", seed=Lk, mask=mask), causal=causal, what=f"{B} {Lq} {Lk} {H} {Hk}")
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_short_axes(D, dtype):
+    """Up to 64 queries and keys, whose gradients one launch forms: shared heads, masks, rows before the first key."""
+    for B, Lq, Lk, H, Hk in ((2, 64, 64, 8, 2), (1, 33, 64, 8, 1), (3, 64, 31, 6, 6), (4, 1, 1, 2, 1), (520, 3, 5, 10, 1), (2, 40, 57, 18, 2)):
+        for causal, mask in ((False, None), (True, None), (False, "random"), (True, "tail")):
+            run(*make(B, Lq, Lk, H, Hk, D, dtype, seed=Lq, mask=mask), causal=causal, scale=0.3, what=f"{B} {Lq} {Lk} {H} {Hk} {causal} {mask}")

@@ -3,7 +3,8 @@
 //   p_ij = exp(s_ij - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
 //   dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i   (dk, dv: over the heads that share them)
 //
-// Two kernels, each the only writer of what it sums, so there are no atomics and the result does not depend on timing:
+// Two kernels (short axes: one, attn_bwd_short_kernel), each the only writer of what it sums, so there are no atomics and the
+// result does not depend on timing:
 // attn_dq_kernel has 32 queries a wave and walks the keys (three products; it also leaves lse in base 2 and delta for the
 // other), attn_dkv_kernel has 32 keys a wave and walks the queries of all heads that share them (four products).  The
 // scores are computed twice that way (7 products instead of 5), the price of having no read-modify-write of dq in memory.
@@ -467,14 +468,178 @@ __global__ void __launch_bounds__(256) attn_dkv_sum_kernel(AttnP p) {
   *reinterpret_cast<bf16x4*>(dst + 4 * part) = y;
 }
 
+// Up to 64 queries and 64 keys: one launch, a workgroup a (batch row, key head).  Both axes lie in LDS whole; waves 0 and 1 have
+// 32 queries each and form dq, waves 2 and 3 have 32 keys each and form dk and dv, over the heads of the group in turn.  The two
+// roles are mirror images: rows of one's own axis in registers, the other axis from LDS.  delta is the sum of the weights times
+// dout . v (the query waves', handed over in LDS), so the forward's rounded out is not read.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) attn_bwd_short_kernel(AttnP p) {
+  constexpr int TB = 64 * D * 2;
+  typedef TileStage<D, 64, 4> Stage;
+  __shared__ __attribute__((aligned(1024))) char buf[4 * TB];            // K, V, Q, dout
+  __shared__ float sl[64], sd[64];                                       // lse in base 2 and delta of the queries
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  const int b = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
+  const bool keys = wave >= 2;
+  const int x0 = 32 * (wave & 1);                                        // this wave's first query or key
+  lds_ptr lds = (lds_ptr)buf;
+  Stage sk, sv, sq, sg;
+  sk.init(lane, wave, p.skl);
+  sv.init(lane, wave, p.svl);
+  sq.init(lane, wave, p.sql);
+  sg.init(lane, wave, p.sgl);
+  auto fetch = [&](int g) {
+    const int hq = hk * p.G + g;
+    sq.load(uni(p.q + b * p.sqb + hq * p.sqh), p.Lq, attn_lds_u32(lds + 2 * TB), wave);
+    sg.load(uni(p.dout + b * p.sgb + hq * p.sgh), p.Lq, attn_lds_u32(lds + 3 * TB), wave);
+    if (wave == 0) {
+      const float x = p.lse[((long long)b * p.H + hq) * p.Lq + min(lane, p.Lq - 1)];
+      sl[lane] = lane >= p.Lq || x == -INFINITY ? INFINITY : x * ATTN_LOG2E;
+    }
+  };
+  uint64_t w = low_bits(p.Lk);
+  if (p.mask) attn_mask_words<1>(p, b, 0, 1, lane, [&](int, uint64_t bits) { w = bits; });
+  w = uni64(w);
+  const char* kb = uni(p.k + b * p.skb + hk * p.skh);
+  const char* vb = uni(p.v + b * p.svb + hk * p.svh);
+  sk.load(kb, p.Lk, w, attn_lds_u32(lds), lane, wave);
+  sv.load(vb, p.Lk, w, attn_lds_u32(lds + TB), lane, wave);
+  fetch(0);
+  TileRead<D> rd;
+  rd.init(lane);
+  lds_cptr mine = lds + (keys ? 0 : 2 * TB), other = lds + (keys ? 2 * TB : 0);      // own axis, the axis that is summed over
+  f32x16 da[D / 32], dv[D / 32];                                         // dq or dk, dv
+  auto clear = [&](f32x16 (&x)[D / 32]) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[i][r] = 0.f;
+  };
+  clear(da);
+  clear(dv);
+  for (int g = 0; g < p.G; ++g) {
+    if (g) {
+      attn_barrier();                                                    // the head before it is done with
+      fetch(g);
+    }
+    attn_barrier();
+    bf16x8 ra[D / 16], rb[D / 16];
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      ra[kk] = rd.row(mine, x0, kk);
+      rb[kk] = rd.row(mine + TB, x0, kk);
+    }
+    f32x16 s[2], dp[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      s[x] = mfma32x32x16<F16>(rd.row(other, 32 * x, 0), ra[0], f32x16{});
+      dp[x] = mfma32x32x16<F16>(rd.row(other + TB, 32 * x, 0), rb[0], f32x16{});
+#pragma unroll
+      for (int kk = 1; kk < D / 16; ++kk) {
+        s[x] = mfma32x32x16<F16>(rd.row(other, 32 * x, kk), ra[kk], s[x]);
+        dp[x] = mfma32x32x16<F16>(rd.row(other + TB, 32 * x, kk), rb[kk], dp[x]);
+      }
+    }
+    if (keys) {
+      const bool keep = (w >> (x0 + n)) & 1;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int first = keep ? (p.causal ? x0 + n - p.off - 32 * x : -64) : 64;    // rows r >= first see this lane's key
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(sl + 32 * x + 8 * u + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * u + e;
+            const float t = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], p.c, -l4[e]));
+            s[x][r] = crow32(r, h) >= first ? t : 0.f;
+          }
+        }
+      }
+    } else {
+      const float lse2 = sl[x0 + n];
+      float d = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t kw = ((uint32_t)(w >> (32 * x)) & (p.causal ? upto(x0 + n + p.off - 32 * x) : ~0u)) >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float t = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], p.c, -lse2));
+          s[x][r] = (kw >> ((r & 3) + 8 * (r >> 2))) & 1 ? t : 0.f;
+          d = __builtin_fmaf(s[x][r], dp[x][r], d);
+        }
+      }
+      d += other_half(d);
+      if (h == 0) sd[x0 + n] = d;
+    }
+    __syncthreads();
+    if (keys) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const bf16x8 pf = attn_pack<F16>(s[x], half);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) dv[i] = mfma32x32x16<F16>(rd.col(other + TB, 32 * x + 16 * half, i), pf, dv[i]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + 32 * x + 8 * u + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[x][4 * u + e] *= dp[x][4 * u + e] - d4[e];
+        }
+      }
+    } else {
+      const float delta = sd[x0 + n];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[x][r] *= dp[x][r] - delta;
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const bf16x8 f = attn_pack<F16>(s[x], half);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) da[i] = mfma32x32x16<F16>(rd.col(other, 32 * x + 16 * half, i), f, da[i]);
+      }
+    if (!keys) {
+      const bool valid = x0 + n < p.Lq;
+      bf16* o = p.dq + b * p.dqb + (long long)(x0 + n) * p.dql + (hk * p.G + g) * p.dqh;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) attn_store<F16>(da[i], p.scale, o + 32 * i, h, valid);
+      clear(da);
+    }
+  }
+  if (keys) {
+    const bool valid = x0 + n < p.Lk;
+    bf16* ok = p.dk + b * p.dkb + (long long)(x0 + n) * p.dkl + hk * p.dkh;
+    bf16* ov = p.dv + b * p.dvb + (long long)(x0 + n) * p.dvl + hk * p.dvh;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      attn_store<F16>(da[i], p.scale, ok + 32 * i, h, valid);
+      attn_store<F16>(dv[i], 1.f, ov + 32 * i, h, valid);
+    }
+  }
+}
+
 struct BwdPlan {
-  bool share;
+  bool share, brief;
   int wq, wk, nbq, nbk, nsplit;
   int64_t gq, gk, stat, part;
 };
 
 BwdPlan bwd_plan(const LrceAttnDesc* d) {
   BwdPlan f{};
+  // one launch for short axes; many heads on few key heads would be left to few workgroups.  Measured (64 x 64, one launch / two
+  // kernels): 600 heads d 64, 40 x 40 11.3 / 15.3 us, 2400 heads d 128 91 / 120, 4 x 32 heads d 128 in groups of 8 18.7 / 20.9, in
+  // groups of 32 (d 64) 67 / 23, 64 x 128 heads in groups of 16 (d 64) 63 / 112
+  f.brief = d->Lq > 0 && d->Lq <= 64 && d->Lk > 0 && d->Lk <= 64 && (d->H / d->Hk <= 8 || (int64_t)d->B * d->Hk >= 512);
+  if (f.brief) {
+    f.gq = (int64_t)d->B * d->Hk;
+    return f;
+  }
   f.wq = d->Lq <= 64 ? 2 : 4;
   f.wk = d->Lk <= 64 ? 2 : 4;
   const int64_t row_tiles = (int64_t)d->B * d->H * ((d->Lq + 31) / 32);
@@ -495,6 +660,10 @@ BwdPlan bwd_plan(const LrceAttnDesc* d) {
 
 template <int D, bool F16>
 void bwd_launch(AttnP p, const BwdPlan& f, hipStream_t s) {
+  if (f.brief) {
+    attn_bwd_short_kernel<D, F16><<<(unsigned)f.gq, 256, 0, s>>>(p);
+    return;
+  }
   if (f.gq) {
     p.nblk = f.nbq;
     if (f.share && f.wq == 2) attn_dq_share_kernel<D, F16, 2><<<(unsigned)f.gq, 128, 0, s>>>(p);
