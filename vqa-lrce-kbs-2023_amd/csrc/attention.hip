@@ -528,7 +528,7 @@ FwdPlan fwd_plan(const LrceAttnDesc* d) {
   f.nsplit = 1;
   const int nt = (d->Lk + 31) / 32;
   const int64_t tiles = (int64_t)d->B * d->Hk * ((rows + 31) / 32);
-  f.split = rows <= 32 || attn_few_rows(tiles, d->Lk);
+  f.split = rows <= 32 || attn_few_rows(tiles, d->Lk, d->D, false);
   if (f.split) {
     f.nblk = (int)((rows + 31) / 32);
     const int64_t base = std::max<int64_t>(1, tiles);

@@ -643,7 +643,7 @@ BwdPlan bwd_plan(const LrceAttnDesc* d) {
   f.wq = d->Lq <= 64 ? 2 : 4;
   f.wk = d->Lk <= 64 ? 2 : 4;
   const int64_t row_tiles = (int64_t)d->B * d->H * ((d->Lq + 31) / 32);
-  f.share = attn_few_rows(row_tiles, d->Lk);
+  f.share = attn_few_rows(row_tiles, d->Lk, d->D, true);
   if (f.share) f.wq = attn_share_waves(d->D, row_tiles);
   f.nbq = f.share ? (d->Lq + 31) / 32 : (d->Lq + 32 * f.wq - 1) / (32 * f.wq);
   f.nbk = (d->Lk + 32 * f.wk - 1) / (32 * f.wk);

@@ -37,8 +37,14 @@ void attn_fill(const LrceAttnDesc* d, AttnP& p);
 
 // Whether the waves of a workgroup share 32 rows and divide the keys, rather than have 32 rows each: where row tiles alone
 // leave the chip's 1024 SIMDs without a second wave to fill the first one's waits, and the key axis is long enough to divide.
-// Measured (64 heads, 1024 keys, d 64, forward): 512 row tiles 10.9 us divided, 21.6 us not; 1024 row tiles 21 us either way.
-inline bool attn_few_rows(int64_t row_tiles, int Lk) { return row_tiles <= 768 && Lk >= 192; }
+// Measured (us divided / not; forward, then dq with dk and dv): 64 heads x 8 tiles x 1024 keys d 64 10.9 / 21.6; 32 heads x 22 tiles
+// x 700 keys d 64 16 / 16, 40 / 40, 32 x 19 x 800 d 32 11 / 14, 25 / 28.  A divided workgroup of the wide heads holds two stages a
+// wave in 49 or 64 KB of LDS: at 64 x 9 x 1213 d 96 30 / 27, 67 / 68, 64 x 8 x 1024 d 96 25 / 22, 47 / 52, and where
+// they are more than the two a CU that fit, 64 x 9 x 1213 d 128 50 / 31, 101 / 87, 32 x 19 x 800 35 / 22, 63 / 55 (32 x 16 x 512 15 / 16,
+// 38 / 42).
+inline bool attn_few_rows(int64_t row_tiles, int Lk, int D, bool bwd) {
+  return Lk >= 192 && row_tiles <= (D <= 64 ? 768 : !bwd ? 500 : D == 96 ? 768 : 512);
+}
 // ... and how many waves: a wave has two stages of K and V of 32 keys in LDS (8 to 32 KB); four waves of the wide ones would
 // leave one workgroup a CU
 inline int attn_share_waves(int D, int64_t row_tiles) { return D <= 64 || row_tiles <= 256 ? 4 : 2; }
