@@ -66,6 +66,24 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// A lane's sums over four columns, rounding by rounding: which products enter an addition unrounded is otherwise the compiler's
+// choice and changes with its flags, and the bf16 operands that follow turn a last bit into a visible one.
+__device__ __forceinline__ float ln_squares(float4 v, float mean) {
+#pragma clang fp contract(off)
+  const float a = v.x - mean, b = v.y - mean, c = v.z - mean, d = v.w - mean;
+  return a * a + b * b + c * c + d * d;
+}
+// sum of a b; p = a b, rounded
+__device__ __forceinline__ float ln_dot(float4 a, float4 b, float4 p) {
+#pragma clang fp contract(off)
+  return __builtin_fmaf(a.z, b.z, __builtin_fmaf(a.x, b.x, p.y)) + p.w;
+}
+__device__ __forceinline__ float ln_dot(float4 a, float4 b) {
+#pragma clang fp contract(off)
+  const float x = a.x * b.x, w = a.w * b.w;
+  return __builtin_fmaf(a.z, b.z, __builtin_fmaf(a.y, b.y, x)) + w;
+}
+
 // CH float4 chunks per lane, LPR lanes per row (rows of <= 128 columns use half a wave each).
 template <typename TX, typename TY, int CH, int LPR>
 __global__ void __launch_bounds__(256) ln_fwd(const TX* x, const int* in_map, int nseg, const float* w, const float* b,
@@ -119,8 +137,7 @@ __global__ void __launch_bounds__(256) ln_fwd(const TX* x, const int* in_map, in
   for (int t = 0; t < CH; ++t) {
     const int c = sl + LPR * t;
     if (c < nch) {
-      const float a = v[t].x - mean, b2 = v[t].y - mean, c2 = v[t].z - mean, d = v[t].w - mean;
-      q += a * a + b2 * b2 + c2 * c2 + d * d;
+      q += ln_squares(v[t], mean);
     }
   }
   const float rstd = rsqrtf(row_sum<LPR>(q) / cols + eps);
@@ -256,8 +273,8 @@ __global__ void __launch_bounds__(256) ln_bwd(const TD* dy, const int* dy_map, c
         const float4 d = dcur[t];
         const float4 ww = wcol[t];
         g[t] = make_float4(d.x * ww.x, d.y * ww.y, d.z * ww.z, d.w * ww.w);
-        s1 += g[t].x + g[t].y + g[t].z + g[t].w;
-        s2 += g[t].x * xh[t].x + g[t].y * xh[t].y + g[t].z * xh[t].z + g[t].w * xh[t].w;
+        s1 += ln_dot(d, ww, g[t]);
+        s2 += ln_dot(g[t], xh[t]);
         aw[t].x += d.x * xh[t].x; aw[t].y += d.y * xh[t].y; aw[t].z += d.z * xh[t].z; aw[t].w += d.w * xh[t].w;
         ab[t].x += d.x; ab[t].y += d.y; ab[t].z += d.z; ab[t].w += d.w;
       }
