@@ -11,8 +11,9 @@
 // leaves the accumulators alone in nearly all tiles.
 //
 // Measured: 2 x 8 heads x 4096 x 4096, d 128, bf16 132 us (1040 TFLOP/s), causal with 2 x 16 heads on 4 147 us (935 TFLOP/s counted,
-// 1008 formed); a plain 8192^3 product 1290 TFLOP/s.  Bound there by the reads of the tiles from LDS (1 KB a matrix instruction) and
-// their waits: without exponentials 133 of 141 us, without LDS reads 110, with nothing but products 103.  At d 32 (48 heads x
+// 1008 formed); a plain 8192^3 product 1290 TFLOP/s.  The matrix pipe is busy 53 % of the cycles there, at a clock that the load
+// holds near 1.7 GHz; LDS 26 %, without bank conflicts.  Bound by the waits for LDS reads (1 KB a matrix instruction) and
+// by the exponentials: without these 133 of 141 us, without LDS reads 110, with nothing but products 103.  At d 32 (48 heads x
 // 1568^2, 41 us) by the vector unit: an exponential and 4 to 5 more instructions a score against 64 multiply-adds.  One token over 32 caches of
 // up to 8190 keys (32 heads on 8, d 128): 147 us, 5.0 TB/s of keys and values.
 //

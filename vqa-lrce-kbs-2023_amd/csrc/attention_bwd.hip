@@ -10,7 +10,8 @@
 // scores are computed twice that way (7 products instead of 5), the price of having no read-modify-write of dq in memory.
 // p and ds are rounded to 16 bits where they become operands; delta and ds are formed in f32.
 // Measured: 2 x 16 heads on 4, 4096 x 4096 causal, d 128, bf16: dq 213 us (3 products, 970 TFLOP/s), dk and dv 347 + 14 us (4 products,
-// 790 TFLOP/s; accumulators and operands of d 128 leave one wave a SIMD, so LDS reads and exponentials are not covered); 48 heads x
+// 790 TFLOP/s; accumulators and operands of d 128 leave one wave a SIMD, so LDS reads and exponentials are not covered: the
+// matrix pipe is busy 41 % of the cycles, 58 % in dq); 48 heads x
 // 1568^2, d 32: 47 + 56 us, the vector unit.  Two waves for 32 keys, one with dv, one with dk, the weights handed over in LDS:
 // the same at d 128 (514 against 518 us of backward), slower below (d 64 533 against 493).
 #include <algorithm>
