@@ -129,3 +129,38 @@ def test_what_the_module_does_not_take():
     turned = w.view(2, 32).t()
     assert b.embedding(ids, turned, 1.0, None, dev, stream) is None and torch.equal(K.embedding(ids, turned), turned[ids])
     assert b.attention(q, k, k, None, False, None, dev + 1, stream) is None
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads_at_once():
+    """Each thread on a stream of its own, through the module: short backward, divided keys, rotation, embedding."""
+    import threading
+    cases = [(2, 40, 40, 4, 2, 64), (1, 1, 5000, 8, 2, 128), (2, 300, 333, 4, 2, 32)]
+    w, pos, f = torch.ones(64, device="cuda"), torch.arange(50, device="cuda"), torch.linspace(1, 0.01, 32, device="cuda")
+    x, ids, tab = gpu(9, 2, 50, 4, 64), torch.arange(700, device="cuda") % 13, gpu(8, 20, 48, dtype=F32)
+
+    def work(i):
+        B, Lq, Lk, H, Hk, D = cases[i % 3]
+        q, k, v = gpu(i, B, Lq, H, D), gpu(i + 10, B, Lk, Hk, D), gpu(i + 20, B, Lk, Hk, D)
+        out, lse = K.attention(q, k, v)
+        return [out, lse, *K.attention_bwd(q, q, k, v, out, lse), *K.qk_norm_rope(x, x, w, w, pos, f),
+                *K.qk_norm_rope_bwd(x, x, x, x, w, w, pos, f), K.embedding(ids, tab), K.embedding_bwd(K.embedding(ids, tab), ids, 20)]
+    want = [work(i) for i in range(6)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def thread(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = work(i)
+                s.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+            s.synchronize()
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -1,9 +1,9 @@
 // The host side of an operator call without an interpreter's share in it: argument test, allocation, descriptor and launch
 // of the attention, norm + rotation and embedding operators for the plain case (strides and alignment as the kernels read
 // them, the tensors' device current).  A call of these on single tokens is host-bound: 12 us each from Python with its
-// descriptor packed there, 6.5 us from here.  Everything else - other layouts, other devices, wrong arguments, errors - returns None, and lrce/kernels.py
-// takes the call, words the refusal or makes the copies.  The launches go through the C ABI, whose addresses bind() gets
-// from the library that Python loaded.
+// descriptor packed there, 6.5 us from here.  Everything else - other layouts, other devices, wrong arguments, errors -
+// returns None, and lrce/kernels.py takes the call, words the refusal or makes the copies.  The launches go through the
+// C ABI, whose addresses bind() gets from the library that Python loaded.
 #include <Python.h>
 
 #include <ATen/ATen.h>
