@@ -118,3 +118,10 @@ def test_short_axes(D, dtype):
     for B, Lq, Lk, H, Hk in ((2, 64, 64, 8, 2), (1, 33, 64, 8, 1), (3, 64, 31, 6, 6), (4, 1, 1, 2, 1), (520, 3, 5, 10, 1), (2, 40, 57, 18, 2)):
         for causal, mask in ((False, None), (True, None), (False, "random"), (True, "tail")):
             run(*make(B, Lq, Lk, H, Hk, D, dtype, seed=Lq, mask=mask), causal=causal, scale=0.3, what=f"{B} {Lq} {Lk} {H} {Hk} {causal} {mask}")
+
+
+def test_few_shares_or_many_rows_over_long_axes():
+    """Where one-wave shares would be few, or their join long, a workgroup's waves have the keys between them; one case each side."""
+    for B, Lq, Lk, H, Hk, D, causal, mask in ((7, 1100, 1100, 1, 1, 32, True, "tail"), (1, 1, 1100, 8, 1, 64, False, None), (1, 1, 3200, 8, 1, 64, True, None),
+                                              (4, 1, 2000, 12, 12, 64, False, "random"), (2, 33, 3000, 8, 2, 128, True, "blocks"), (1, 200, 4000, 8, 8, 96, True, None)):
+        run(*make(B, Lq, Lk, H, Hk, D, "bf16", seed=Lk, mask=mask), causal=causal, what=f"{B} {Lq} {Lk} {H} {Hk} {D}")

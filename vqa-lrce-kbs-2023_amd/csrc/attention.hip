@@ -541,10 +541,13 @@ FwdPlan fwd_plan(const LrceAttnDesc* d) {
     const int64_t base = std::max<int64_t>(1, tiles);
     f.waves = attn_share_waves(d->D, base);
     f.split_tiles = std::max(2, (nt + 1) / 2 * 2);
-    if (nt > 32 && base < 512) {
-      // one-wave shares of at least 16 tiles, about two and a half times as many as are resident (LDS: two stages of K and V)
-      const int64_t resident = 256 * std::min<int64_t>(8, 160 * 1024 / (256 * d->D + 512));
-      const int n = (int)std::max<int64_t>(1, std::min<int64_t>((5 * resident / 2 + base - 1) / base, nt / 16));
+    // one-wave shares of at least 16 tiles, about two and a half times as many as are resident (LDS: two stages of K and V), where
+    // they cut the keys finer than the waves of one workgroup would and the join has few rows (7 heads x 1468 x 1468 d 32: 56 us in
+    // two shares, 37 of them the join, 14 by four waves; 8 x 8 heads on 2, 16 rows, 4096 keys d 128: 26 and 38 us; 32 x 32 heads on 8,
+    // one row, d 128: 147 and 174 us over up to 8190 keys, 201 and 180 where all caches have 8190)
+    const int64_t resident = 256 * std::min<int64_t>(8, 160 * 1024 / (256 * d->D + 512));
+    const int n = (int)std::max<int64_t>(1, std::min<int64_t>((5 * resident / 2 + base - 1) / base, nt / 16));
+    if (nt > 32 && base < 512 && n > f.waves && (int64_t)d->B * d->H * d->Lq <= d->Lk) {
       f.waves = 1;
       f.split_tiles = ((nt + n - 1) / n + 1) / 2 * 2;
       f.nsplit = (nt + f.split_tiles - 1) / f.split_tiles;
