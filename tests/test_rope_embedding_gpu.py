@@ -109,6 +109,17 @@ def test_norm_rope_heads(H, Hk):
     rope_case(1, 9, H, Hk, 128, 64, "f32", True, seed=2, start=10 ** 6)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("eps", [0.0, 1e-50])
+def test_norm_rope_without_eps(eps, dtype):
+    """eps = 0, or one that is 0 in 32 bits: lanes without a head (12 of 16, 2 of 8) or without a token add nothing to the weights'
+    gradients."""
+    rope_case(2, 37, 12, 12, 64, 64, dtype, False, eps=eps)
+    rope_case(2, 37, 8, 2, 128, 64, dtype, True, eps=eps)
+    rope_case(1, 5, 1, 1, 32, 32, dtype, False, eps=eps)
+    rope_case(1, 3, 3, 1, 136, 70, dtype, False, eps=eps)
+
+
 def test_norm_rope_zero_rows_and_alignment():
     """Rows of zeros: the norm is held by eps; an odd start of the rows takes narrower loads, not wrong ones."""
     g = torch.Generator(device=dev).manual_seed(5)

@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(256, BWD ? (VEC == 8 ? 3 : 4) : 5) qk_rope_ker
             ss += __shfl_xor(ss, o, 64);
             sg_ += __shfl_xor(sg_, o, 64);
           }
-          const float r = 1.f / sqrtf(ss * inv_d + p.eps), m = sg_ * r * inv_d;   // m = mean(g w xhat)
+          // (a group without a head or a token has ss = 0: with eps = 0 its 0 / 0 would reach the weights' gradients)
+          const float r = act ? 1.f / sqrtf(ss * inv_d + p.eps) : 0.f, m = sg_ * r * inv_d;   // m = mean(g w xhat)
 #pragma unroll
           for (int c = 0; c < NCH; ++c) {
             float o[W];
