@@ -125,3 +125,15 @@ def test_few_shares_or_many_rows_over_long_axes():
     for B, Lq, Lk, H, Hk, D, causal, mask in ((7, 1100, 1100, 1, 1, 32, True, "tail"), (1, 1, 1100, 8, 1, 64, False, None), (1, 1, 3200, 8, 1, 64, True, None),
                                               (4, 1, 2000, 12, 12, 64, False, "random"), (2, 33, 3000, 8, 2, 128, True, "blocks"), (1, 200, 4000, 8, 8, 96, True, None)):
         run(*make(B, Lq, Lk, H, Hk, D, "bf16", seed=Lk, mask=mask), causal=causal, what=f"{B} {Lq} {Lk} {H} {Hk} {D}")
+
+
+def test_one_row_over_more_than_256_shares():
+    """The join takes 256 shares at a time; some of them, the first among them, see nothing."""
+    Lk, H, D = 200001, 2, 32
+    assert K()._attn_ws(False, 1, H, 1, 1, Lk, D) > 256 * H * (D + 2)
+    q, k, v, do, _ = make(1, 1, Lk, H, 1, D, "bf16", seed=11)
+    m = torch.rand(1, Lk, generator=torch.Generator(device=dev).manual_seed(12), device=dev) < 0.4
+    for a, b in ((0, 1500), (60000, 63000), (150000, 199990)):
+        m[:, a:b] = False
+    for mask in (m, None):
+        run(q, k, v, do, mask, what=f"mask={mask is not None}")

@@ -120,6 +120,15 @@ def test_norm_rope_without_eps(eps, dtype):
     rope_case(1, 3, 3, 1, 136, 70, dtype, False, eps=eps)
 
 
+@pytest.mark.parametrize("B,L,H,Hk,D,R,dtype,inter", [
+    (2, 5003, 12, 2, 64, 64, "bf16", False), (2, 5003, 3, 3, 40, 40, "f16", True), (1, 9001, 4, 1, 96, 32, "f32", True), (1, 50011, 1, 1, 64, 64, "bf16", False)])
+def test_norm_rope_of_more_tokens_than_are_resident(B, L, H, Hk, D, R, dtype, inter):
+    """Over 4 x 768 (eight values a load) or 4 x 1024 waves' tokens: the backward's waves take several tokens each, the last ones fewer
+    than the grid.  A weight gradient is then at most 4 tokens of one head in a lane, 6 exchanges, 3 waves and 16 + 6 sums of
+    workgroups: below the 128 additions that the allowance counts."""
+    rope_case(B, L, H, Hk, D, R, dtype, inter)
+
+
 def test_norm_rope_zero_rows_and_alignment():
     """Rows of zeros: the norm is held by eps; an odd start of the rows takes narrower loads, not wrong ones."""
     g = torch.Generator(device=dev).manual_seed(5)
