@@ -429,7 +429,7 @@ int lrce_qk_norm_rope_bwd(const LrceRopeDesc* desc, void* stream);
 /* Embedding lookup y[i][:] = scale * w[ids[i]][:] (types 0 bf16, 1 fp16, 2 f32; y has w's type, or any where w is f32; ids int32 /
  * int64 (ids_bytes 4 / 8); an id outside [0, rows) gives a row of NaN) and its gradient dw[v][:] (f32 [rows][cols], contiguous)
  * = (accumulate: +=) scale * sum over ids[i] = v of dy[i][:], in token order (tokens sorted by id, no atomics on the sums: the
- * same bits each time); ids outside the table and padding_idx (-1: none) have no gradient. */
+ * same bits each time); ids outside the table and the row padding_idx (below rows; -1: none) have no gradient. */
 int lrce_embedding_fwd(const void* ids, int ids_bytes, int64_t n, const void* w, int64_t ld_w, int64_t rows, int cols, int w_type,
                        void* y, int y_type, float scale, void* stream);
 int64_t lrce_embedding_bwd_workspace(int64_t n, int64_t rows, int cols);

@@ -147,3 +147,18 @@ def test_operators_shapes():
     assert y.shape == (3, 4, 24) and y.dtype == torch.float16
     dw = torch.ops.lrce.embedding_backward(y, ids, 100)
     assert dw.shape == (100, 24) and dw.dtype == torch.float32
+
+
+def test_padding_idx_is_a_row_or_none():
+    """-1: none; what nn.Embedding would count from the end, or refuse, is refused."""
+    from lrce import _native as N
+    from lrce import ops  # noqa: F401  (registers the ops)
+    _, L = lib()
+    for pad, rc in ((-2, 1), (-10, 1), (10, 1), (1 << 40, 1), (-1, 0), (0, 0), (9, 0)):
+        assert L.lrce_embedding_bwd(A, 8, 0, A, 2, A, 10, 16, 1.0, pad, 1, None, 0, None) == rc, pad   # (no token: nothing is launched)
+        assert rc == 0 or b"padding_idx" in L.lrce_last_error()
+        if rc:
+            with pytest.raises(N.NativeError, match="padding_idx"):
+                torch.ops.lrce.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(10, 16), 1.0, pad)
+            with pytest.raises(N.NativeError, match="padding_idx"):
+                torch.ops.lrce.embedding_backward(torch.zeros(3, 16), torch.zeros(3, dtype=torch.int64), 10, 1.0, pad)

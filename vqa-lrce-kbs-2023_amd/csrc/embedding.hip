@@ -511,6 +511,7 @@ extern "C" int lrce_embedding_bwd(const void* ids, int ids_bytes, int64_t n, con
   if (n < 0 || n >= (1ll << 31) || rows < 1 || cols < 1 || rows >= (1ll << 31)) return lrce_fail(LRCE_E_ARG, "embedding_bwd: bad sizes n=%lld rows=%lld cols=%d", (long long)n, (long long)rows, cols);
   if (ids_bytes != 4 && ids_bytes != 8) return lrce_fail(LRCE_E_ARG, "embedding_bwd: ids of %d bytes (4 or 8)", ids_bytes);
   if (dy_type < 0 || dy_type > 2) return lrce_fail(LRCE_E_ARG, "embedding_bwd: type %d", dy_type);
+  if (padding_idx < -1 || padding_idx >= rows) return lrce_fail(LRCE_E_ARG, "embedding_bwd: padding_idx %lld of %lld rows (-1: none)", (long long)padding_idx, (long long)rows);
   if (!dw || reinterpret_cast<uintptr_t>(dw) % 16) return lrce_fail(LRCE_E_ARG, "embedding_bwd: dw must start at a multiple of 16 bytes");
   if (n > 0 && (!ids || !dy)) return lrce_fail(LRCE_E_ARG, "embedding_bwd: null pointer");
   if (n == 0 && accumulate) return LRCE_OK;

@@ -937,13 +937,19 @@ def _embed_ws(n, rows, cols):
     return N.lib().lrce_embedding_bwd_workspace(n, rows, cols)
 
 
+def check_padding(what, padding_idx, rows):
+    if not -1 <= padding_idx < rows:
+        raise N.NativeError(f"{what}: padding_idx {padding_idx} of {rows} rows (-1: none; not counted from the end)")
+
+
 def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=-1, dw=None):
     """The gradient of embedding()'s table for dy [*ids.shape, cols] (bf16, fp16 or f32): f32 [rows, cols], row v = scale * the sum
-    of dy over the places where ids is v, in their order (the same bits each time); padding_idx (-1: none) and ids outside the
-    table have none.  dw: a contiguous f32 [rows, cols] the gradient is added to (and returned) instead of a new tensor."""
+    of dy over the places where ids is v, in their order (the same bits each time); the row padding_idx (-1: none; not counted from
+    the end) and ids outside the table have none.  dw: a contiguous f32 [rows, cols] the gradient is added to (and returned) instead of a new tensor."""
     b, dev, stream = _direct(dy) if dw is None else (None, 0, 0)
     if b and (r := b.embedding_bwd(dy, ids, rows, scale, padding_idx, dev, stream)) is not None:
         return r
+    check_padding("embedding_bwd", padding_idx, rows)
     if not (dy.is_cuda and dy.dtype in _TYPE):
         _chk(dy, None, "embedding_bwd: dy")
         raise N.NativeError(f"embedding_bwd: dy must be bf16, fp16 or f32, got {dy.dtype}")

@@ -384,7 +384,10 @@ qk_norm_rope.register_autograd(_rope_backward, setup_context=_rope_setup)
 
 @torch.library.custom_op("lrce::embedding", mutates_args=())
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int = -1) -> Tensor:
-    """scale * weight[ids] (lrce_embedding_fwd); padding_idx: the row without a gradient (-1: none), as nn.Embedding's."""
+    """scale * weight[ids] (lrce_embedding_fwd); padding_idx: the row without a gradient, as nn.Embedding's, but not counted from the
+    end: -1 is none, and below -1 or past the table is refused."""
+    if padding_idx != -1:
+        K.check_padding("embedding", padding_idx, weight.shape[0])
     return K.embedding(ids, weight, scale)
 
 
