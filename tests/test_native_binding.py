@@ -29,6 +29,18 @@ def test_the_module_takes_nothing_from_the_host():
         b.bind(*[0] * 10)
 
 
+def test_the_module_is_built_for_torchs_abi(tmp_path):
+    """The compile line has the loading interpreter's torch and its C++ ABI, not the compiler's default."""
+    import os
+    import subprocess
+    import sys
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(N.__file__)))), "csrc")
+    out = str(tmp_path / "b.so")
+    line = subprocess.run(["make", "-s", "-C", csrc, "-B", "CXX=echo", "PYTHON=" + sys.executable, "BINDING=" + out, out], check=True,
+                          capture_output=True, text=True).stdout
+    assert f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())} " in line and f"-I{os.path.dirname(torch.__file__)}/include" in line
+
+
 def gpu(seed, *shape, dtype=BF):
     return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)
 
