@@ -368,3 +368,22 @@ def test_refusals():
         with pytest.raises(N.NativeError):
             call()
             pytest.fail(f"call {i} was accepted")
+
+
+@pytest.mark.parametrize("Lq,Lk,H,D", [(1, 20000, 8, 64), (1, 600, 8, 64), (3, 700, 4, 128), (300, 600, 4, 32), (900, 64, 4, 64)])
+def test_what_is_seen_under_a_weight_of_zero_is_not_lost(Lq, Lk, H, D):
+    """A visible v of NaN or infinity whose key lies 128 below the row's maximum (a weight of 0 in 32 bits): 0 x NaN, by whatever split
+    of the keys - shares joined, waves joined, one walk."""
+    q = torch.full((1, Lq, H, D), 4.0, dtype=BF, device=dev)
+    k, v = torch.zeros(1, Lk, 2, D, dtype=BF, device=dev), rnd(1, 1, Lk, 2, D)
+    k[:, -1] = 128 / (4.0 * D ** 0.5)
+    for bad in (math.nan, math.inf):
+        w = v.clone()
+        w[0, 3, 1, 5] = bad
+        out, lse = K().attention(q, k, w)
+        assert not torch.isfinite(out[0, :, H // 2:, 5]).any()
+        out[0, :, H // 2:, 5] = 0
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+        m = torch.ones(1, Lk, dtype=torch.bool, device=dev)
+        m[0, 3] = False
+        assert torch.isfinite(K().attention(q, k, w, key_mask=m)[0]).all()

@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_fwd_kernel(AttnP p) {
   if (valid && h == 0) p.lse[(long long)bh * p.Lq + row] = l == 0.f ? -INFINITY : st.m * p.scale + __logf(l);
 }
 
-// What a share (maximum m, sum l) counts at the common maximum mx; a share that saw nothing counts nothing
+// What a share (maximum m, sum l) counts at the common maximum mx; a share that saw nothing (its sums are zeros) counts nothing.
+// A factor that underflows to 0 is multiplied all the same: a NaN among the share's values stays one, as within a share.
 __device__ __forceinline__ float join_factor(float m, float l, float mx, float c) {
   return m == -INFINITY && l == 0.f ? 0.f : l != l ? l : __builtin_amdgcn_exp2f((m - mx) * c);
 }
@@ -391,11 +392,9 @@ __global__ void __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) attn_split_kernel(At
     for (int w = 0; w < NW; ++w) {
       const float a = join_factor(sm[w][rr], sl[w][rr], mx, p.c);
       const float* src = reinterpret_cast<float*>(buf) + (w * 32 + rr) * OP + part * DP;
-      if (a != 0.f) {
-        ls += a * sl[w][rr];
+      ls += a * sl[w][rr];
 #pragma unroll
-        for (int e = 0; e < DP; ++e) o[e] += a * src[e];
-      }
+      for (int e = 0; e < DP; ++e) o[e] += a * src[e];
     }
     const int gi = gr / p.G, gh = hk * p.G + gr % p.G;
     const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
@@ -436,15 +435,14 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnP p) {
       const float2 ml = *reinterpret_cast<const float2*>(p.ws2 + 2 * ((c0 + threadIdx.x) * rows + row));
       const float a = join_factor(ml.x, ml.y, mx, p.c);
       sa[threadIdx.x] = a;
-      if (a != 0.f) ls += a * ml.y;
+      ls += a * ml.y;
     }
     __syncthreads();
     if (g < GR) {
 #pragma unroll 8
       for (int s = g; s < n; s += GR) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(p.ws + ((c0 + s) * rows + row) * D + 4 * part);
-        const float a = sa[s];
-        if (a != 0.f) o += a * x;
+        o += sa[s] * x;
       }
     }
   }
