@@ -129,6 +129,26 @@ def test_norm_rope_of_more_tokens_than_are_resident(B, L, H, Hk, D, R, dtype, in
     rope_case(B, L, H, Hk, D, R, dtype, inter)
 
 
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotation_of_far_positions(inter):
+    """Rows whose only value is sqrt(64) (root mean square 1, each rounding but the angle's exact): the rotated pair is the cosine and the
+    sine, each right to 3 units of its own size, near their zeros too.  The angle's three roundings in 64 bits, and the reference's
+    one, are 4 x 2^-53 of it; 2^-44: the two terms of an angle's sine where they cancel."""
+    L, D = 4001, 64
+    pos = torch.cat([torch.arange(2000, device=dev), 2 ** 20 + 7 * torch.arange(2001, device=dev)])
+    freq = (10000.0 ** (-torch.arange(32, device=dev, dtype=F64) / 32)).float()
+    x = torch.zeros(1, L, 32, D, device=dev)
+    first = 2 * torch.arange(32, device=dev) if inter else torch.arange(32, device=dev)
+    second = first + (1 if inter else 32)
+    x[0, :, torch.arange(32, device=dev), first] = 8.0
+    w = torch.ones(D, device=dev)
+    y, _ = K().qk_norm_rope(x, x[:, :, :1], w, w, pos, freq, eps=0.0, interleaved=inter)
+    ang = pos.to(F64)[:, None] * freq.to(F64)
+    i = torch.arange(32, device=dev)
+    for got, want in ((y[0, :, i, first], ang.cos()), (y[0, :, i, second], ang.sin())):
+        near(got / 8, want, 3 * 2.0 ** -23 * want.abs() + 4 * 2.0 ** -53 * ang + 2.0 ** -44, "cosine or sine")
+
+
 def test_norm_rope_zero_rows_and_alignment():
     """Rows of zeros: the norm is held by eps; an odd start of the rows takes narrower loads, not wrong ones."""
     g = torch.Generator(device=dev).manual_seed(5)

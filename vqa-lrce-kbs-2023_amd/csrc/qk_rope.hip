@@ -8,8 +8,8 @@
 // has VEC pairs of a row (two vectors of VEC values), a power of two of lanes a row, so a row's sums are a few shuffles;
 // a wave has one token (or several, where its heads are few) and walks the token's heads, query heads first, so the angles are
 // formed once a token.  They are formed as turns in 64 bits (position * frequency / 2 pi less its nearest integer): far
-// positions lose nothing, and the sine and cosine of the remainder need no range reduction.  All arithmetic on the values is
-// f32, rounded once.  The weight gradients are summed in registers over a workgroup's tokens, across its lanes in LDS, and
+// positions lose nothing, and the sine and cosine of the remainder, f32 values, need no range reduction.  All arithmetic on the
+// values is f32, rounded once.  The weight gradients are summed in registers over a workgroup's tokens, across its lanes in LDS, and
 // over the workgroups by a second kernel in a fixed order.
 // Measured: 4 x 8192 tokens of 32 + 8 heads, d 128, bf16: forward 116 us (671 MB, 5.8 TB/s), backward 204 + 5 us (1.0 GB, 4.9 TB/s);
 // 10 x 333 tokens of 8 + 8 heads, d 96, f32: 10.7 us, 16.4 + 4.2 us.  The next tokens' rows fetched ahead cost registers and
@@ -101,8 +101,13 @@ struct Pairs {
     if (on && pi < p.R / 2) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const double turns = position * (double)p.freq[pi + i] * PER_TURN;
-        sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &sn[i], &cs[i]);
+        const double turns = position * (double)p.freq[pi + i] * PER_TURN, x = 2.0 * (turns - __builtin_rint(turns));
+        // x in f32 is up to 2^-25 half turns off, 1e-7 radians; the rest of it is added to first order (the second is below 2^-47)
+        const float near = (float)x, rest = (float)(x - (double)near) * 3.14159265f;
+        float s, c;
+        sincospif(near, &s, &c);
+        sn[i] = __builtin_fmaf(c, rest, s);
+        cs[i] = __builtin_fmaf(-s, rest, c);
       }
     }
   }
