@@ -387,3 +387,42 @@ def test_what_is_seen_under_a_weight_of_zero_is_not_lost(Lq, Lk, H, D):
         m = torch.ones(1, Lk, dtype=torch.bool, device=dev)
         m[0, 3] = False
         assert torch.isfinite(K().attention(q, k, w, key_mask=m)[0]).all()
+
+
+def operator_calls():
+    g = torch.Generator(device=dev).manual_seed(21)
+    q, k, v = rnd(1, 2, 40, 4, 64), rnd(2, 2, 70, 2, 64), rnd(3, 2, 70, 2, 64)
+    m = torch.rand(2, 70, generator=g, device=dev) < 0.7
+    w, kw, f = rnd(4, 64, dtype=torch.float32), rnd(5, 64, dtype=torch.float32), torch.linspace(1, 0.01, 20, device=dev)
+    pos, ids = torch.arange(40, device=dev), torch.randint(0, 50, (2, 40), generator=g, device=dev)
+    return (("attention", (q, k, v, m, True, 0.2)), ("qk_norm_rope", (q, k[:, :40], w, kw, pos, f, 1e-5, True)),
+            ("embedding", (ids, rnd(6, 50, 64), 2.0, 3)))
+
+
+def test_autograd_is_the_backward_calls():
+    """The gradients that autograd hands out are the backward calls' own, bit for bit; integers, masks and frequencies have none."""
+    for name, args in operator_calls():
+        live = [a.clone().requires_grad_() if torch.is_tensor(a) and a.is_floating_point() else a for a in args]
+        if name == "qk_norm_rope":
+            live[5] = args[5]
+        y = getattr(ops(), name)(*live)
+        outs = [t for t in (y if isinstance(y, tuple) else (y,)) if t.requires_grad]
+        dy = [rnd(30 + i, *t.shape, dtype=t.dtype) for i, t in enumerate(outs)]
+        got = torch.autograd.grad(outs, [t for t in live if torch.is_tensor(t) and t.requires_grad], dy)
+        if name == "attention":
+            q, k, v, m, causal, scale = args
+            want = K().attention_bwd(dy[0], q, k, v, *K().attention(q, k, v, m, causal, scale), m, causal, scale)
+        elif name == "qk_norm_rope":
+            want = K().qk_norm_rope_bwd(*dy, *args)
+        else:
+            want = (K().embedding_bwd(dy[0], args[0], 50, args[2], args[3]).to(BF),)
+        assert len(got) == len(want)
+        for a, b in zip(got, want):
+            assert a.dtype == b.dtype and torch.equal(a, b), name
+
+
+def test_operators_keep_the_dispatchers_rules():
+    """Schemas, shapes without data, and autograd by torch's own check."""
+    for name, args in operator_calls():
+        live = [a.clone().requires_grad_() if torch.is_tensor(a) and a.is_floating_point() and a.dim() > 1 else a for a in args]
+        torch.library.opcheck(getattr(ops(), name).default, tuple(live))
