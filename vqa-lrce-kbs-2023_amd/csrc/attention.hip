@@ -6,12 +6,13 @@
 // over the keys that row i may see; a row that sees none gives o = 0, lse = -inf.  One pass over the keys with a
 // running maximum and sum in f32.  S^T = K Q^T, so a lane owns one query: the row statistics are in-lane plus one
 // exchange of the wave's halves, and P^T, rounded to 16 bits (half a unit in the last place of each weight, the size
-// of the output's own rounding), is at once the B operand of O^T += V^T P^T.  The running maximum is raised only when a
+// of the output's own rounding: the output's error is 1.2 - 1.4 times what f32 weights leave), is at once the B operand of
+// O^T += V^T P^T.  The running maximum is raised only when a
 // tile exceeds it by more than 2^8 (the weights then stay below 2^8, harmless in f32 and in both 16-bit types), which
 // leaves the accumulators alone in nearly all tiles.
 //
 // Measured: 2 x 8 heads x 4096 x 4096, d 128, bf16 132 us (1040 TFLOP/s), causal with 2 x 16 heads on 4 147 us (935 TFLOP/s counted,
-// 1008 formed); a plain 8192^3 product 1290 TFLOP/s.  The matrix pipe is busy 53 % of the cycles there, at a clock that the load
+// 1008 formed; 165 in a loop of nothing else, where the clock falls); a plain 8192^3 product 1290 TFLOP/s.  The matrix pipe is busy 53 % of the cycles there, at a clock that the load
 // holds near 1.7 GHz; LDS 26 %, without bank conflicts.  Bound by the waits for LDS reads (1 KB a matrix instruction) and
 // by the exponentials: without these 133 of 141 us, without LDS reads 110, with nothing but products 103.  At d 32 (48 heads x
 // 1568^2, 41 us) by the vector unit: an exponential and 4 to 5 more instructions a score against 64 multiply-adds.  One token over 32 caches of
@@ -542,7 +543,9 @@ FwdPlan fwd_plan(const LrceAttnDesc* d) {
     // one-wave shares of at least 16 tiles, about two and a half times as many as are resident (LDS: two stages of K and V), where
     // they cut the keys finer than the waves of one workgroup would and the join has few rows (7 heads x 1468 x 1468 d 32: 56 us in
     // two shares, 37 of them the join, 14 by four waves; 8 x 8 heads on 2, 16 rows, 4096 keys d 128: 26 and 38 us; 32 x 32 heads on 8,
-    // one row, d 128: 147 and 174 us over up to 8190 keys, 201 and 180 where all caches have 8190)
+    // one row, d 128: 147 and 174 us over up to 8190 keys).  It is set for caches of different fill; the mask is not looked at, and
+    // where all caches are full, masked or not, the last takes 196 - 201 us, 180 by four waves.  B H Lq <= Lk is where the first of
+    // these is told from the others: the join reads that many rows a share
     const int64_t resident = 256 * std::min<int64_t>(8, 160 * 1024 / (256 * d->D + 512));
     const int n = (int)std::max<int64_t>(1, std::min<int64_t>((5 * resident / 2 + base - 1) / base, nt / 16));
     if (nt > 32 && base < 512 && n > f.waves && (int64_t)d->B * d->H * d->Lq <= d->Lk) {

@@ -8,12 +8,15 @@
 // attn_dq_kernel has 32 queries a wave and walks the keys (three products; it also leaves lse in base 2 and delta for the
 // other), attn_dkv_kernel has 32 keys a wave and walks the queries of all heads that share them (four products).  The
 // scores are computed twice that way (7 products instead of 5), the price of having no read-modify-write of dq in memory.
-// p and ds are rounded to 16 bits where they become operands; delta and ds are formed in f32.
-// Measured: 2 x 16 heads on 4, 4096 x 4096 causal, d 128, bf16: dq 213 us (3 products, 970 TFLOP/s), dk and dv 347 + 14 us (4 products,
-// 790 TFLOP/s; accumulators and operands of d 128 leave one wave a SIMD, so LDS reads and exponentials are not covered: the
-// matrix pipe is busy 41 % of the cycles, 58 % in dq); 48 heads x
-// 1568^2, d 32: 47 + 56 us, the vector unit.  Two waves for 32 keys, one with dv, one with dk, the weights handed over in LDS:
-// the same at d 128 (514 against 518 us of backward), slower below (d 64 533 against 493).
+// p and ds are rounded to 16 bits where they become operands (the matrix instructions that take f32 have a sixteenth of the
+// rate); delta and ds are formed in f32.  With the forward's rounded weights this makes the gradients' error 1.4 times what f32
+// weights leave.  In fp16 a ds above 65504 becomes infinite and one below 2^-25 is lost: the loss scale has to leave
+// p |dout . v - delta| between.
+// Measured: 2 x 16 heads on 4, 4096 x 4096 causal, d 128, bf16: 516 - 553 us as the clock under matrix load goes, of it dq 204 - 226 (3
+// products, 910 - 1010 TFLOP/s), dk and dv 301 - 347 + 14 (4 products, 790 - 910; accumulators and operands of d 128 leave one wave a
+// SIMD, so LDS reads and exponentials are not covered: the matrix pipe is busy 41 % of the cycles, 58 % in dq); 48 heads x 1568^2,
+// d 32: 47 + 56 us, the vector unit.  Two waves for 32 keys, one with dv, one with dk, the weights handed over in LDS: the same at
+// d 128 (514 against 518 us of backward, both in turn), slower below (d 64 533 against 493).
 #include <algorithm>
 
 #include "attention_util.h"

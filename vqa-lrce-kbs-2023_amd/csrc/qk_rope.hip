@@ -11,8 +11,8 @@
 // positions lose nothing, and the sine and cosine of the remainder, f32 values, need no range reduction.  All arithmetic on the
 // values is f32, rounded once.  The weight gradients are summed in registers over a workgroup's tokens, across its lanes in LDS, and
 // over the workgroups by a second kernel in a fixed order.
-// Measured: 4 x 8192 tokens of 32 + 8 heads, d 128, bf16: forward 116 us (671 MB, 5.8 TB/s), backward 204 + 5 us (1.0 GB, 4.9 TB/s);
-// 10 x 333 tokens of 8 + 8 heads, d 96, f32: 10.7 us, 16.4 + 4.2 us.  The next tokens' rows fetched ahead cost registers and
+// Measured: 4 x 8192 tokens of 32 + 8 heads, d 128, bf16: forward 117 us (671 MB, 5.7 TB/s), backward 206 + 5 us (1.0 GB, 4.9 TB/s);
+// 10 x 333 tokens of 8 + 8 heads, d 96, f32: 10.8 us, 17.0 + 4.1 us.  The next tokens' rows fetched ahead cost registers and
 // so waves: 133 and 232 us at the first size.
 #include <algorithm>
 #include <cmath>

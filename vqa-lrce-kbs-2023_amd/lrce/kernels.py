@@ -781,7 +781,9 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
 
 def attention_bwd(dout, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
     """(dq, dk, dv) of attention() for dout, with the forward's out and lse; the arguments as there.  Sums over the query
-    heads that share a key head are formed in f32; the result does not depend on timing."""
+    heads that share a key head are formed in f32; the result does not depend on timing.  The weights p and
+    ds = p (dout . v - delta) are matrix operands in q's type: in fp16 a ds above 65504 becomes infinite and one below 2^-25 is
+    lost, so dout wants a loss scale between."""
     b, dev, stream = _direct(q)
     if b and (r := b.attention_bwd(q, k, v, key_mask, causal, scale, dout, out, lse, dev, stream)):
         return r

@@ -45,7 +45,8 @@ differentiable through the same native kernels (linear: dX / dW GEMMs + fused bi
 layer_norm: lrce_layernorm_bwd w.r.t. y; window_attention: window_attention_backward w.r.t. out —
 its qkv / lse outputs are saved activations, marked non-differentiable; patch_embed: w.r.t. the conv
 and LayerNorm parameters, the clips are data; attention: attention_backward w.r.t. out, lse is a saved
-activation, marked non-differentiable; qk_norm_rope and embedding: their backward ops).  decoder_recurrent is a forward (inference) op; the
+activation, marked non-differentiable; qk_norm_rope and embedding: their backward ops; positions, frequencies, masks
+and ids have no gradient; a 16-bit embedding table takes one more pass over its gradient, f32 -> its type).  decoder_recurrent is a forward (inference) op; the
 model's training path differentiates the decoder as one autograd node (lrce/models/fusionv3.py).
 """
 from typing import List, Optional, Tuple
