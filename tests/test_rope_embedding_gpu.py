@@ -221,3 +221,15 @@ def test_embedding_ids_outside_the_table_and_shapes():
 def test_embedding_of_many_tokens_and_wide_tables(N, V, C):
     """More than 2^18 tokens (more places a workgroup), ids of 19 and 20 bits (three passes of the sort)."""
     test_embedding(N, V, C, ("f32", "f32", "f32"))
+
+
+def test_padding_idx_outside_the_table_is_refused():
+    from lrce import _native as N, ops  # noqa: F401  (registers the ops)
+    w, ids = torch.randn(10, 16, device=dev, requires_grad=True), torch.tensor([3, 9, 0], device=dev)
+    for pad in (-2, -10, 10):
+        for call in (lambda: K().embedding_bwd(w.detach()[:3], ids, 10, padding_idx=pad), lambda: torch.ops.lrce.embedding(ids, w, 1.0, pad),
+                     lambda: K().embedding_bwd(w.detach()[:3], ids, 10, padding_idx=pad, dw=torch.zeros(10, 16, device=dev))):
+            with pytest.raises(N.NativeError, match="padding_idx"):
+                call()
+    torch.ops.lrce.embedding(ids, w, 1.0, 9).sum().backward()
+    assert (w.grad[9] == 0).all() and (w.grad[[0, 3]] == 1).all()
